@@ -287,6 +287,80 @@ int b200k_attention_batch(float *out, const float *q, const void *kc, const void
                           int32_t scratch_positions, int32_t nh, int32_t nkv, int32_t hs, int32_t half,
                           b200fwd_stream stream);
 
+/* ---- the paged 8-bit cache: keys and values of many requests in blocks of a shared pool, half a float16 cache's bytes
+ * (no counterpart in the reference, whose cache is one float32 or float16 run of positions: forward.js:269-289).
+ *
+ * The pool: values int8 [blocks][nkv][block][hs] and one float32 scale per (block, kv head) [blocks][nkv], for keys
+ * (kc, ks) and for values (vc, vs); a stored value stands for its integer times its scale. `block` positions a block:
+ * a multiple of 16, 16 to 256; hs a multiple of 16, 16 to 256; nkv 1 to 1024; blocks * block below 2^31. Caches and
+ * rows start on 16 bytes (strides in elements; a multiple of 4 floats or 8 float16). `half`: rows are float16 bits,
+ * else float32. A request's positions sit in the blocks that its row of `tables` ([n_seqs][table_width] block ids)
+ * names in order: position p in slot tables[i][p / block] * block + p % block.
+ *
+ * Calls only enqueue kernels and allocate nothing, so they can be captured into a graph. Everything they read on the
+ * device is looked over there: an id, slot or offset that is out of range is never followed. */
+
+/* One step of the requests' tables: request i goes from lengths[i] to max(0, lengths[i] + news[i]) positions. news[i]
+ * > 0 appends (blocks are taken from the ring of free ids, in the order of the requests), < 0 takes positions back,
+ * all of them where it is -lengths[i] or less: blocks that are left are put at the ring's tail. (Where the new length
+ * ends inside a block, that block stays, and its scale: b200k_cache8_store.)
+ * ring: [blocks] ids, the free ones at state[0], state[0] + 1, ... (modulo blocks), state[1] of them.
+ * Written: tables (the new blocks' entries), ring (blocks given back), lengths_out [n_seqs], state_out [4] {the ring's
+ * head, its free ids, a status, the step's tokens}; and for a step's buffers of n rows: starts [n_seqs + 1], request i's
+ * tokens are rows starts[i]..starts[i + 1] - 1; slots, seq and pos [n], each token's slot, request and position (seq and
+ * pos may be NULL), -1 in rows behind the last token. lengths_out may be lengths and state_out state (updated in
+ * place); no other two arrays may overlap.
+ * All or nothing: where the status is not 0, lengths, tables, ring, head and count stay, and the step has no tokens. */
+#define B200K_TABLES_BLOCKS 1 /* too few free blocks */
+#define B200K_TABLES_TOKENS 2 /* more than n tokens */
+#define B200K_TABLES_WIDTH 3  /* a request longer than its table row */
+#define B200K_TABLES_INPUT 4  /* a length or a state that cannot be */
+int b200k_block_tables(int32_t *tables, int32_t *ring, int32_t *state_out, int32_t *lengths_out, int32_t *starts,
+                       int32_t *slots, int32_t *seq, int32_t *pos, const int32_t *state, const int32_t *lengths,
+                       const int32_t *news, int32_t n_seqs, int32_t table_width, int32_t blocks, int32_t block,
+                       int32_t n, b200fwd_stream stream);
+/* Keys and values k, v (n rows of nkv * hs, k_stride and v_stride elements apart) into their slots; rows with a slot
+ * that is none are left out. A block's tokens stand next to one another in the call, in the order of their slots, each
+ * slot once. A (block, head)'s scale is the float32 nearest to max |x| / 127 over all its values (earlier ones by the
+ * scale that they had), the integers are nearest to x / scale, half to even. Positions before the first one stored now
+ * are the block's earlier tokens: where the scale grows, their integers go to the new step the same way, q * old / new.
+ * Storing position 0 of a block begins it anew. A value that is no finite number makes the (block, head)'s scale NaN
+ * and its new integers 0: it reads as NaN until the block is begun anew. */
+int b200k_cache8_store(int8_t *kc, float *ks, int8_t *vc, float *vs, const void *k, const void *v,
+                       const int32_t *slots, int32_t n, int64_t k_stride, int64_t v_stride, int32_t blocks,
+                       int32_t block, int32_t nkv, int32_t hs, int32_t half, b200fwd_stream stream);
+/* What slots hold, integer times scale in float32 (rounded to float16 where half), into n rows of k and v; rows with a
+ * slot that is none are left as they were. (b200fwd_keys_values for this cache.) */
+int b200k_cache8_load(void *k, void *v, const int8_t *kc, const float *ks, const int8_t *vc, const float *vs,
+                      const int32_t *slots, int32_t n, int64_t k_stride, int64_t v_stride, int32_t blocks,
+                      int32_t block, int32_t nkv, int32_t hs, int32_t half, b200fwd_stream stream);
+/* Attention of n query rows (nh heads of hs; q_stride, out_stride elements apart) over the cache: request i's tokens are
+ * rows starts[i]..starts[i + 1] - 1, the last of its lengths[i] positions, and each sees the positions up to its own:
+ * b200k_attention's softmax(q . k / sqrt(hs)) v, for blocks of tokens and single ones in one call (what
+ * b200k_block_tables leaves in starts, lengths_out and tables). Query head h reads kv head h / (nh / nkv). A row that
+ * sees no position (fewer positions than tokens) is 0; a row that sees a position whose table entry is no block, or
+ * past its table row, is NaN. Rows that belong to no request are left as they were; starts that do not ascend within
+ * 0..n leave out unwritten. Not to the bit like b200k_attention, but within float32's rounding (half: float16's) of the
+ * exact result for the stored values; the same call gives the same bits. Up to 65536 requests, n * nh up to 2^30,
+ * table_width * block up to 2^30. scratch: b200k_cache8_attention_scratch() bytes of device memory, 256-byte aligned,
+ * nothing zeroed; calls that overlap on the GPU need one each. */
+int b200k_cache8_attention(void *out, const void *q, const int8_t *kc, const float *ks, const int8_t *vc,
+                           const float *vs, const int32_t *tables, const int32_t *starts, const int32_t *lengths,
+                           int32_t n, int32_t n_seqs, int32_t table_width, int32_t blocks, int32_t block, int32_t nh,
+                           int32_t nkv, int32_t hs, int64_t q_stride, int64_t out_stride, int32_t half, void *scratch,
+                           b200fwd_stream stream);
+int b200k_cache8_attention_scratch(int32_t n, int32_t n_seqs, int32_t nh, int32_t nkv, int32_t hs, int32_t half,
+                                   uint64_t *bytes);
+/* What a sampler's answer is reported with, of `count` rows of n logits (stride elements apart; float16 where half):
+ * logprob[r] = log softmax(row r)[targets[r]] (NaN where the target is no id; NULL: not wanted), entropy[r] = -sum p log p
+ * in nats (NULL: not wanted), and the k (0 to 32) most probable ids with their log probabilities, top_id and top_logprob
+ * [count][k], the largest first, ties by the lowest id. Masked logits may be -inf (log probability -inf) or any lowest
+ * value. A row without a finite largest logit (all -inf, or an infinity or a NaN in it) gives NaN and ids -1. Float32
+ * arithmetic whatever the logits; no scratch. */
+int b200k_logprobs(float *logprob, float *entropy, float *top_logprob, int32_t *top_id, const void *logits,
+                   const int32_t *targets, int32_t count, int32_t n, int64_t stride, int32_t k, int32_t half,
+                   b200fwd_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

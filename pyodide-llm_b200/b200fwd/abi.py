@@ -13,6 +13,9 @@ TENSOR_ABSENT, TENSOR_INT8, TENSOR_F32, TENSOR_F16 = 0, 1, 2, 3
 KINDS = {"int8": TENSOR_INT8, "f32": TENSOR_F32, "f16": TENSOR_F16}
 MAX_OUTLIERS = 16
 
+# what b200k_block_tables leaves in state_out[2]
+TABLES_BLOCKS, TABLES_TOKENS, TABLES_WIDTH, TABLES_INPUT = 1, 2, 3, 4
+
 OK, EINVAL, ECUDA, ENOMEM, EUNSUPPORTED, ENOTFINITE, ETIMEOUT = 0, -1, -2, -3, -4, -5, -6
 
 
@@ -168,6 +171,13 @@ def load():
                                   I32, P, P),
         "b200k_attention_batch": (P, P, P, P, P, P, P, I32, I64, I32, I32, I32, I32, I32, P),
         "b200k_matmul_plan": (I32, I32, I32, I32, I32, P, P),
+        "b200k_block_tables": (P, P, P, P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, P),
+        "b200k_cache8_store": (P, P, P, P, P, P, P, I32, I64, I64, I32, I32, I32, I32, I32, P),
+        "b200k_cache8_load": (P, P, P, P, P, P, P, I32, I64, I64, I32, I32, I32, I32, I32, P),
+        "b200k_cache8_attention": (P, P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, I32, I32, I32, I64, I64, I32, P,
+                                   P),
+        "b200k_cache8_attention_scratch": (I32, I32, I32, I32, I32, I32, ctypes.POINTER(U64)),
+        "b200k_logprobs": (P, P, P, P, P, P, I32, I32, I64, I32, I32, P),
     }
     for name, args in sig.items():
         fn = getattr(lib, name)

@@ -1,0 +1,749 @@
+// cache8_attention.cu — attention over the paged 8-bit cache (cache8.cu), for single tokens and blocks of tokens of
+// many requests at once: out = sum_j p_j v_j, p = softmax_j(q . k_j / sqrt(hs)) over the positions j up to the row's
+// own, k_j = kscale[block][head] * int8, v_j likewise.
+//
+// A tile is RT (8 or 16) query rows of one request and kv head: its tokens' query heads that share the kv head, so
+// every byte of the cache is read once for all of them. The products run on mma.sync m16n8k16 (float16 operands,
+// float32 sums) with the cache as the 16-row operand: int8 integers are exact in float16, and the scales stay outside
+// (a block's key scale on its scores, its value scale within its weights), so the cache's values are never rounded.
+// Single tokens are bound by the cache's bytes; the tensor instructions' rate is no limit there.
+//  - float32 queries: q and the weights each as a float16 pair high + low (22 bits), two instructions for one;
+//    float16 queries are exact, and their weights are rounded to the same pairs: the outputs' own rounding remains.
+//  - weights: w = 2^(s + log2(vscale) - M), M a running maximum (per row) that moves only when it is passed by more
+//    than 2^8, and the row sum l += w / vscale: the block's value scale costs no operation per value, and what is
+//    rounded to float16 is relative to the largest term of the sum, whatever the scales.
+// Work is split over the length of the caches: the tiles' units of 16 positions, laid end to end, are cut into equal
+// spans, one for each thread block of a grid that fills the GPU once, so ragged requests balance and one long request
+// takes every SM. A tile cut by a span's end leaves partial sums (unnormalized, with M and l) that combine_kernel
+// joins in the order of the spans: results don't depend on timing.
+// Loads: each lane copies the bytes that it will multiply itself (cp.async into a ring of its own, so no thread waits
+// for another), stages deep enough to cover HBM's latency.
+#include <cuda_fp16.h>
+
+#include <cstdint>
+#include <string>
+
+#include "cache8.h"
+#include "common.h"
+
+namespace b200 {
+namespace {
+
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int UNIT = 16;          // positions of a unit: one operand tile, within one block of the cache
+constexpr int RING = 16384;       // bytes of a warp's ring
+constexpr float RESCALE = 8.0f;   // log2 of how far a weight may rise above 1 before M moves
+constexpr int MOST_BLOCKS = 148 * 3;  // thread blocks of a grid (resident at once)
+
+struct Args {
+  void *out;
+  const void *q;
+  const int8_t *kc, *vc;
+  const float *ks, *vs;
+  const int32_t *tables, *starts, *lengths;
+  int4 *meta;       // [tiles] {first span, spans, request, row tile}; meta[-1].x: the tiles
+  float2 *part_ml;  // [span + tile][kv head][RT] {M, l}
+  float *part;      // [span + tile][kv head][RT][hs]
+  int64_t q_stride, out_stride;
+  int n, n_seqs, width, blocks, block, nkv, hs, group, min_units;
+  int64_t most_tiles;
+  float scale;      // log2(e) / sqrt(hs)
+};
+
+// request i of the call: its first row, its rows, and its positions (all of them, the new ones included)
+struct Request {
+  int first, fresh, length;
+};
+__device__ __forceinline__ Request request_of(const Args &a, int i) {
+  const int s0 = min(max(a.starts[i], 0), a.n), s1 = min(max(a.starts[i + 1], s0), a.n);
+  return {s0, s1 - s0, max(a.lengths[i], 0)};
+}
+template <int RT>
+__device__ __forceinline__ int tiles_of(const Args &a, const Request &r) {
+  return (r.fresh * a.group + RT - 1) / RT;
+}
+// its units: the positions that its table has room for, one unit at least (a row that sees nothing is written too)
+__device__ __forceinline__ int units_of(const Args &a, const Request &r) {
+  return max(1, (min(r.length, a.width * a.block) + UNIT - 1) / UNIT);
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+// BYTES (4, 8 or 16) to shared memory, zeros where !on (then nothing is read)
+template <int BYTES>
+__device__ __forceinline__ void copy(uint32_t dst, const void *src, bool on) {
+  if (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(on ? BYTES : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2 *>(&u)); }
+// two of a word's bytes (already + 128) as float16 integers: 1024 + b is a float16 whose low byte is b
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t widen(uint32_t biased) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(biased), "r"(0x64646464u), "n"(SEL));
+  const __half2 v = __hsub2(*reinterpret_cast<__half2 *>(&d), __half2half2(__ushort_as_half(0x6480)));  // less 1152
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t interleave_lo(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5140); }
+__device__ __forceinline__ uint32_t interleave_hi(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7362); }
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// sums of {work units, tiles} over the requests before this thread's (one request a thread), and of all
+__device__ __forceinline__ void block_scan(int64_t (&v)[2], int64_t (&all)[2], int64_t (*part)[WARPS]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t own[2] = {v[0], v[1]};
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, v[j], d);
+      if (lane >= d) v[j] += o;
+    }
+  __syncthreads();
+  if (lane == 31) part[0][warp] = v[0], part[1][warp] = v[1];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    all[j] = 0;
+    int64_t before = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      if (w < warp) before += part[j][w];
+      all[j] += part[j][w];
+    }
+    v[j] += before - own[j];
+  }
+}
+
+template <int HSEG, int RT, bool HALF>
+struct Shape {
+  static constexpr int HP = HSEG * 64;              // the head size, padded
+  static constexpr int NT = RT / 8;                 // row tiles of the instruction
+  static constexpr int KSTEPS = HSEG * 4;           // instructions along the head
+  static constexpr int VB = HSEG % 2 ? 8 : 16;      // bytes of a lane's piece of a value row
+  static constexpr int VN = HP / (8 * VB);          // pieces
+  static constexpr int STAGE = HSEG * 2048;         // bytes of a unit's keys and values
+  static constexpr int STAGES = RING / STAGE;       // 8, 4, 2, 2
+  static constexpr int QREGS = KSTEPS * NT * (HALF ? 2 : 4);
+  static constexpr bool QREG = QREGS <= 32;         // the query fragments in registers, else in shared memory
+  static constexpr int MINB = HSEG * RT <= 16 ? 3 : 2;
+  struct Smem {
+    alignas(16) uint8_t ring[WARPS][RING];          // later the warps' sums [WARPS][RT][HP]
+    alignas(16) uint4 qf[QREG ? 1 : KSTEPS * NT * 32];
+    float sc[WARPS][STAGES][2];                     // the units' scales
+    float ml[WARPS][RT][2];
+    int64_t part[2][WARPS];
+    int64_t found[3];
+  };
+};
+
+template <int HSEG, int RT, bool HALF>
+__global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8_attention_kernel(const Args a) {
+  using S = Shape<HSEG, RT, HALF>;
+  constexpr int NT = S::NT, HP = S::HP, STAGES = S::STAGES;
+  extern __shared__ __align__(16) uint8_t raw[];
+  typename S::Smem &sm = *reinterpret_cast<typename S::Smem *>(raw);
+  pdl_begin();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  const int h = blockIdx.y;
+
+  // ---- this block's span of the units
+  int64_t total = 0, all_tiles = 0;
+  for (int i = tid; i < a.n_seqs; i += THREADS) {
+    const Request r = request_of(a, i);
+    all_tiles += tiles_of<RT>(a, r);
+    total += (int64_t)tiles_of<RT>(a, r) * units_of(a, r);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, d);
+    all_tiles += __shfl_xor_sync(0xffffffffu, all_tiles, d);
+  }
+  if (lane == 0) sm.part[0][warp] = total, sm.part[1][warp] = all_tiles;
+  __syncthreads();
+  total = sm.part[0][0] + sm.part[0][1] + sm.part[0][2] + sm.part[0][3];
+  all_tiles = sm.part[1][0] + sm.part[1][1] + sm.part[1][2] + sm.part[1][3];
+  if (all_tiles > a.most_tiles) total = 0;  // starts that don't ascend: rows of several requests, nothing is written
+  const int64_t span = max((int64_t)a.min_units, (total + gridDim.x - 1) / gridDim.x);
+  int64_t at = span * blockIdx.x;
+  const int64_t end = min(at + span, total);
+  if (at >= end) {
+    if (total == 0 && blockIdx.x == 0 && h == 0 && tid == 0) a.meta[-1] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  // ---- the request in which it begins; {units, tiles} before that request
+  int64_t before[2] = {0, 0};
+  int req = 0;
+  {
+    int64_t carry[2] = {0, 0};
+    for (int base = 0; base < a.n_seqs; base += THREADS) {
+      const int i = base + tid;
+      int64_t v[2] = {0, 0}, all[2], w = 0;
+      if (i < a.n_seqs) {
+        const Request r = request_of(a, i);
+        v[1] = tiles_of<RT>(a, r);
+        w = v[0] = v[1] * units_of(a, r);
+      }
+      block_scan(v, all, sm.part);
+      if (w && carry[0] + v[0] <= at && at < carry[0] + v[0] + w) {
+        sm.found[0] = carry[0] + v[0];
+        sm.found[1] = carry[1] + v[1];
+        sm.found[2] = i;
+      }
+      carry[0] += all[0], carry[1] += all[1];
+    }
+    __syncthreads();
+    before[0] = sm.found[0], before[1] = sm.found[1], req = (int)sm.found[2];
+    if (blockIdx.x == 0 && h == 0 && tid == 0) a.meta[-1] = make_int4((int)carry[1], 0, 0, 0);
+  }
+
+  const uint32_t ring = smem_u32(sm.ring[warp]);
+  uint8_t *ring_p = sm.ring[warp];
+  while (at < end) {
+    const Request r = request_of(a, req);
+    const int tiles = tiles_of<RT>(a, r), units = units_of(a, r);
+    if (tiles == 0) {
+      req++;
+      continue;
+    }
+    const int tile = (int)((at - before[0]) / units), u0 = (int)((at - before[0]) % units);
+    const int u1 = (int)min((int64_t)units, u0 + (end - at));
+    const int64_t tile_at = before[0] + (int64_t)tile * units;
+    const int span0 = (int)(tile_at / span), spans = (int)((tile_at + units - 1) / span) - span0 + 1;
+    const int64_t tile_id = before[1] + tile;
+    if (h == 0 && tid == 0 && u0 == 0) a.meta[tile_id] = make_int4(span0, spans, req, tile);
+
+    // ---- the tile's rows: row x is query head x % group of the kv head, of the request's token x / group
+    const int rows = r.fresh * a.group, x0 = tile * RT, cap = a.width * a.block;
+    const int last = r.length - r.fresh + (min(rows, x0 + RT) - 1) / a.group;  // the last row's position
+    const int first = r.length - r.fresh + x0 / a.group;                       // the first row's
+    const int u_end = min(u1, (min(last + 1, cap) + UNIT - 1) / UNIT);         // no row sees further units
+
+    // query fragments: lane (g, c) holds, for row g of row tile t, the head's values 64 j + 16 c + 4 w .. + 3
+    uint32_t qh[S::QREG ? S::KSTEPS * NT : 1][2], ql[S::QREG && !HALF ? S::KSTEPS * NT : 1][2];
+    float qf[NT][2];  // what the scores of this lane's columns (rows 2 c, 2 c + 1 of row tile t) are to be scaled by
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const int x = x0 + 8 * t + g;
+      const bool on = x < rows;
+      const int64_t off = (int64_t)(r.first + (on ? x / a.group : 0)) * a.q_stride +
+                          (int64_t)(h * a.group + (on ? x % a.group : 0)) * a.hs;
+      float f = 1.0f, back = 1.0f;
+      if (!HALF) {
+        // each row by a power of two into (0, 2): float16 holds 22 bits of it in two parts
+        const float *src = reinterpret_cast<const float *>(a.q) + off;
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < HSEG; j++) {
+          const int d = 64 * j + 16 * c;
+          if (on && d < a.hs) {
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+              const float4 v = *reinterpret_cast<const float4 *>(src + d + 4 * w);
+              top = fmaxf(fmaxf(fmaxf(top, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+            }
+          }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
+        f = __uint_as_float((uint32_t)(127 - e) << 23);
+        back = __uint_as_float((uint32_t)(127 + e) << 23);
+      }
+      qf[t][0] = __shfl_sync(0xffffffffu, back, 8 * c) * a.scale;
+      qf[t][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4) * a.scale;
+#pragma unroll
+      for (int j = 0; j < HSEG; j++) {
+        const int d = 64 * j + 16 * c;
+        const bool in = on && d < a.hs;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+          if (in) {
+            if (HALF) {
+              const uint2 v = *reinterpret_cast<const uint2 *>(reinterpret_cast<const __half *>(a.q) + off + d + 4 * w);
+              hi[0] = v.x, hi[1] = v.y;
+            } else {
+              const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + off + d + 4 * w);
+              const float y[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+#pragma unroll
+              for (int p = 0; p < 2; p++) {
+                hi[p] = pack(y[2 * p], y[2 * p + 1]);
+                const float2 back2 = unpack(hi[p]);
+                lo[p] = pack(y[2 * p] - back2.x, y[2 * p + 1] - back2.y);
+              }
+            }
+          }
+          const int k = (4 * j + w) * NT + t;
+          if (S::QREG) {
+            qh[S::QREG ? k : 0][0] = hi[0], qh[S::QREG ? k : 0][1] = hi[1];
+            if (!HALF) ql[S::QREG && !HALF ? k : 0][0] = lo[0], ql[S::QREG && !HALF ? k : 0][1] = lo[1];
+          } else if (warp == 0) {
+            sm.qf[S::QREG ? 0 : k * 32 + lane] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+          }
+        }
+      }
+    }
+    int pos[NT][2];  // the positions of this lane's columns (-1: no row)
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        const int x = x0 + 8 * t + 2 * c + p;
+        pos[t][p] = x < rows ? r.length - r.fresh + x / a.group : -1;
+      }
+    if (!S::QREG) __syncthreads();
+
+    // ---- the units of this warp: u0 + warp, + WARPS, ...
+    float M[NT][2], l[NT][2], o[NT][HSEG * 4][4];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      M[t][0] = M[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.0f;
+#pragma unroll
+      for (int m = 0; m < HSEG * 4; m++) o[t][m][0] = o[t][m][1] = o[t][m][2] = o[t][m][3] = 0.0f;
+    }
+    const int32_t *table = a.tables + (int64_t)req * a.width;
+    auto page_of = [&](int u) { return u < u_end ? table[u * UNIT / a.block] : -1; };
+    auto issue = [&](int u, int slot, int page) {
+      if (u < u_end) {
+        const bool ok = page >= 0 && page < a.blocks;
+        const int64_t ph = ok ? (int64_t)page * a.nkv + h : 0;
+        const int64_t row = ph * a.block + u * UNIT % a.block;
+        const uint32_t dst = ring + slot * S::STAGE + lane * 16;
+#pragma unroll
+        for (int y = 0; y < 2; y++)
+#pragma unroll
+          for (int j = 0; j < HSEG; j++) {
+            const int d = 64 * j + 16 * c;
+            const bool on = ok && d < a.hs;
+            copy<16>(dst + (y * HSEG + j) * 512, a.kc + (row + g + 8 * y) * a.hs + (on ? d : 0), on);
+          }
+        const uint32_t vdst = ring + slot * S::STAGE + HSEG * 1024 + lane * S::VB;
+#pragma unroll
+        for (int y = 0; y < 4; y++)
+#pragma unroll
+          for (int p = 0; p < S::VN; p++) {
+            const int d = p * 8 * S::VB + S::VB * g;
+            const bool on = ok && d < a.hs;
+            copy<S::VB>(vdst + (y * S::VN + p) * 32 * S::VB,
+                        a.vc + (row + 2 * c + (y & 1) + 8 * (y >> 1)) * a.hs + (on ? d : 0), on);
+          }
+        // a table entry that is no block of the pool: NaN scales, so every row that sees it comes out NaN
+        if (lane < 2) {
+          float *dst_s = &sm.sc[warp][slot][lane];
+          if (ok) copy<4>(smem_u32(dst_s), (lane ? a.vs : a.ks) + ph, true);
+          else *dst_s = __uint_as_float(0x7fffffffu);
+        }
+      }
+      copies_commit();
+    };
+    {
+      int u = u0 + warp;
+      int pages[STAGES];
+#pragma unroll
+      for (int s = 0; s < STAGES; s++) pages[s] = page_of(u + s * WARPS);
+#pragma unroll
+      for (int s = 0; s < STAGES - 1; s++) issue(u + s * WARPS, s, pages[s]);
+      int next = pages[STAGES - 1], slot = 0;
+      for (; u < u_end; u += WARPS) {
+        copies_wait<STAGES - 2>();
+        __syncwarp();
+        const float kscale = sm.sc[warp][slot][0], vscale = sm.sc[warp][slot][1];
+        // ---- scores: S^T = K Q^T, 16 positions x 8 rows an instruction tile
+        float s[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+        const uint8_t *base = ring_p + slot * S::STAGE;
+#pragma unroll
+        for (int j = 0; j < HSEG; j++) {
+          const uint4 k0 = *reinterpret_cast<const uint4 *>(base + j * 512 + lane * 16);
+          const uint4 k1 = *reinterpret_cast<const uint4 *>(base + (HSEG + j) * 512 + lane * 16);
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            const uint32_t y0 = w0[w] ^ 0x80808080u, y1 = w1[w] ^ 0x80808080u;
+            const uint32_t a0 = widen<0x4140>(y0), a1 = widen<0x4140>(y1), a2 = widen<0x4342>(y0), a3 = widen<0x4342>(y1);
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+              const int k = (4 * j + w) * NT + t;
+              if (S::QREG) {
+                mma(s[t], a0, a1, a2, a3, qh[S::QREG ? k : 0][0], qh[S::QREG ? k : 0][1]);
+                if (!HALF) mma(s[t], a0, a1, a2, a3, ql[S::QREG && !HALF ? k : 0][0], ql[S::QREG && !HALF ? k : 0][1]);
+              } else {
+                const uint4 f = sm.qf[S::QREG ? 0 : k * 32 + lane];
+                mma(s[t], a0, a1, a2, a3, f.x, f.y);
+                if (!HALF) mma(s[t], a0, a1, a2, a3, f.z, f.w);
+              }
+            }
+          }
+        }
+        // ---- weights. A value scale below 2^-100 counts as 2^-100 (a block of zeros has scale 0): what it weighs
+        // is below any other block's last place
+        const float vs = !(vscale < 7.888609e-31f) ? vscale : 7.888609e-31f;
+        const float lg = __log2f(vs), inv = __fdiv_rn(1.0f, vs);
+        const bool masked = u * UNIT + UNIT - 1 > first;
+        bool up = false;
+        float f[NT][2];
+        bool on[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+          for (int p = 0; p < 2; p++) f[t][p] = kscale * qf[t][p];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            on[t][e] = !masked || u * UNIT + g + 8 * (e >> 1) <= pos[t][e & 1];
+            up |= on[t][e] && __fmaf_rn(s[t][e], f[t][e & 1], lg) > M[t][e & 1] + RESCALE;
+          }
+        }
+        if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+              float m = fmaxf(on[t][p] ? __fmaf_rn(s[t][p], f[t][p], lg) : -INFINITY,
+                              on[t][2 + p] ? __fmaf_rn(s[t][2 + p], f[t][p], lg) : -INFINITY);
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+              m = fmaxf(m, M[t][p]);
+              const float by = M[t][p] == m ? 1.0f : ex2(M[t][p] - m);
+              l[t][p] *= by;
+#pragma unroll
+              for (int x = 0; x < HSEG * 4; x++) o[t][x][p] *= by, o[t][x][2 + p] *= by;
+              M[t][p] = m;
+            }
+        }
+        uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float m = M[t][e & 1] == -INFINITY ? 0.0f : M[t][e & 1];
+            w[e] = on[t][e] ? ex2(__fmaf_rn(s[t][e], f[t][e & 1], lg - m)) : 0.0f;
+          }
+          // (a row that sees nothing of the unit: 0 times a scale that may be NaN)
+          l[t][0] = __fmaf_rn(w[0] + w[2], on[t][0] || on[t][2] ? inv : 0.0f, l[t][0]);
+          l[t][1] = __fmaf_rn(w[1] + w[3], on[t][1] || on[t][3] ? inv : 0.0f, l[t][1]);
+#pragma unroll
+          for (int y = 0; y < 2; y++) {
+            const uint32_t hi = pack(w[2 * y], w[2 * y + 1]);
+            const float2 b = unpack(hi);
+            ph[t][y] = transposed(hi);
+            pl[t][y] = transposed(pack(w[2 * y] - b.x, w[2 * y + 1] - b.y));
+          }
+        }
+        // ---- O^T += V^T P^T: lane (g, c)'s pieces of the rows of positions 2c, 2c + 1, 2c + 8, 2c + 9
+        const uint8_t *vbase = base + HSEG * 1024 + lane * S::VB;
+#pragma unroll
+        for (int p = 0; p < S::VN; p++) {
+          uint32_t vw[4][S::VB / 4];
+#pragma unroll
+          for (int y = 0; y < 4; y++) {
+            const uint8_t *src = vbase + (y * S::VN + p) * 32 * S::VB;
+            if (S::VB == 16) {
+              const uint4 v = *reinterpret_cast<const uint4 *>(src);
+              vw[y][0] = v.x, vw[y][1] = v.y, vw[y][S::VB / 4 - 2] = v.z, vw[y][S::VB / 4 - 1] = v.w;
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2 *>(src);
+              vw[y][0] = v.x, vw[y][1] = v.y;
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < S::VB / 4; w++)
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+              const uint32_t p0 = (y ? interleave_hi(vw[0][w], vw[1][w]) : interleave_lo(vw[0][w], vw[1][w])) ^ 0x80808080u;
+              const uint32_t p1 = (y ? interleave_hi(vw[2][w], vw[3][w]) : interleave_lo(vw[2][w], vw[3][w])) ^ 0x80808080u;
+              const uint32_t a0 = widen<0x4140>(p0), a1 = widen<0x4342>(p0), a2 = widen<0x4140>(p1), a3 = widen<0x4342>(p1);
+              const int m = p * S::VB / 2 + 2 * w + y;
+#pragma unroll
+              for (int t = 0; t < NT; t++) {
+                mma(o[t][m], a0, a1, a2, a3, ph[t][0], ph[t][1]);
+                mma(o[t][m], a0, a1, a2, a3, pl[t][0], pl[t][1]);
+              }
+            }
+        }
+        __syncwarp();  // every lane has read the slot's scales
+        const int ahead = u + (STAGES - 1) * WARPS;
+        issue(ahead, slot == 0 ? STAGES - 1 : slot - 1, next);
+        next = page_of(ahead + WARPS);
+        slot = slot + 1 == STAGES ? 0 : slot + 1;
+      }
+      copies_wait<0>();
+    }
+
+    // ---- the four warps' sums to one M a row, then added in the warps' order
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        l[t][p] += __shfl_xor_sync(0xffffffffu, l[t][p], 4);
+        l[t][p] += __shfl_xor_sync(0xffffffffu, l[t][p], 8);
+        l[t][p] += __shfl_xor_sync(0xffffffffu, l[t][p], 16);
+        if (g == 0) sm.ml[warp][8 * t + 2 * c + p][0] = M[t][p], sm.ml[warp][8 * t + 2 * c + p][1] = l[t][p];
+      }
+    __syncthreads();
+    float *sums = reinterpret_cast<float *>(sm.ring);
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        const int x = 8 * t + 2 * c + p;
+        float top = sm.ml[0][x][0];
+#pragma unroll
+        for (int w = 1; w < WARPS; w++) top = fmaxf(top, sm.ml[w][x][0]);
+        const float by = M[t][p] == top ? 1.0f : ex2(M[t][p] - top);
+        float *dst = sums + ((int64_t)warp * RT + x) * HP;
+#pragma unroll
+        for (int q = 0; q < S::VN; q++)
+#pragma unroll
+          for (int w = 0; w < S::VB / 4; w++) {
+            const int m = q * S::VB / 2 + 2 * w;
+            *reinterpret_cast<float4 *>(dst + q * 8 * S::VB + S::VB * g + 4 * w) = make_float4(
+                o[t][m][p] * by, o[t][m][2 + p] * by, o[t][m + 1][p] * by, o[t][m + 1][2 + p] * by);
+          }
+      }
+    __syncthreads();
+    const int quads = a.hs / 4;
+    for (int i = tid; i < RT * quads; i += THREADS) {
+      const int x = i / quads, d = (i - x * quads) * 4;
+      if (x0 + x >= rows) break;
+      float top = sm.ml[0][x][0], sum_l = 0.0f;
+#pragma unroll
+      for (int w = 1; w < WARPS; w++) top = fmaxf(top, sm.ml[w][x][0]);
+      float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) {
+        const float m = sm.ml[w][x][0];
+        sum_l += sm.ml[w][x][1] * (m == top ? 1.0f : ex2(m - top));
+        const float4 v = *reinterpret_cast<const float4 *>(sums + ((int64_t)w * RT + x) * HP + d);
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+      }
+      const int token = (x0 + x) / a.group, head = h * a.group + (x0 + x) % a.group;
+      if (r.length - r.fresh + token >= cap) sum_l = __uint_as_float(0x7fffffffu);  // positions past the table's row
+      if (spans == 1) {
+        const float by = sum_l == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum_l);
+        const int64_t off = (int64_t)(r.first + token) * a.out_stride + (int64_t)head * a.hs + d;
+        if (HALF) {
+          *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(a.out) + off) =
+              make_uint2(pack(sum.x * by, sum.y * by), pack(sum.z * by, sum.w * by));
+        } else {
+          *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + off) =
+              make_float4(sum.x * by, sum.y * by, sum.z * by, sum.w * by);
+        }
+      } else {
+        const int64_t row = ((blockIdx.x + tile_id) * a.nkv + h) * RT + x;
+        *reinterpret_cast<float4 *>(a.part + row * a.hs + d) = sum;
+        if (d == 0) a.part_ml[row] = make_float2(top, sum_l);
+      }
+    }
+    at += u1 - u0;
+    if (tile + 1 == tiles && u1 == units) {
+      before[0] += (int64_t)tiles * units;
+      before[1] += tiles;
+      req++;
+    }
+  }
+}
+
+// one row of a tile that several spans have worked on: its partial sums joined, in the spans' order within each warp
+// and the warps' at the end
+constexpr int CW = 4;  // warps
+template <int RT, bool HALF>
+__global__ void __launch_bounds__(CW * 32) cache8_combine_kernel(const Args a) {
+  pdl_begin();
+  __shared__ float acc[CW][256], ml[CW][2];
+  const int tile_id = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (tile_id >= a.meta[-1].x) return;
+  const int4 meta = a.meta[tile_id];
+  if (meta.y < 2) return;
+  const Request r = request_of(a, meta.z);
+  for (int x = blockIdx.z; x < RT; x += gridDim.z) {
+    const int row_of = meta.w * RT + x;
+    if (row_of >= r.fresh * a.group) break;
+    float M = -INFINITY, l = 0.0f, o[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) o[j] = 0.0f;
+    for (int s = warp; s < meta.y; s += CW) {
+      const int64_t row = (((int64_t)meta.x + s + tile_id) * a.nkv + h) * RT + x;
+      const float2 v = a.part_ml[row];
+      const float m = fmaxf(M, v.x), by = M == m ? 1.0f : ex2(M - m), vy = v.x == m ? 1.0f : ex2(v.x - m);
+      l = l * by + v.y * vy;
+      M = m;
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (lane + 32 * j < a.hs) o[j] = o[j] * by + a.part[row * a.hs + lane + 32 * j] * vy;
+    }
+    if (lane == 0) ml[warp][0] = M, ml[warp][1] = l;
+#pragma unroll
+    for (int j = 0; j < 8; j++) acc[warp][lane + 32 * j] = o[j];
+    __syncthreads();
+    float top = ml[0][0], sum_l = 0.0f, by[CW];
+#pragma unroll
+    for (int w = 1; w < CW; w++) top = fmaxf(top, ml[w][0]);
+#pragma unroll
+    for (int w = 0; w < CW; w++) {
+      by[w] = ml[w][0] == top ? 1.0f : ex2(ml[w][0] - top);
+      sum_l += ml[w][1] * by[w];
+    }
+    const float f = sum_l == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum_l);
+    const int token = row_of / a.group, head = h * a.group + row_of % a.group;
+    const int64_t off = (int64_t)(r.first + token) * a.out_stride + (int64_t)head * a.hs;
+    for (int d = threadIdx.x; d < a.hs; d += CW * 32) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < CW; w++) sum += acc[w][d] * by[w];
+      if (HALF) reinterpret_cast<__half *>(a.out)[off + d] = __float2half_rn(sum * f);
+      else reinterpret_cast<float *>(a.out)[off + d] = sum * f;
+    }
+    __syncthreads();  // acc and ml have been read
+  }
+}
+
+// rows of a tile: 8 where the requests have that few on average, else 16 (a row tile costs instructions whether its
+// rows are there or not; a request with more rows takes several tiles)
+int rows_of_tile(int n, int n_seqs, int group) { return (int64_t)n * group <= 8 * (int64_t)n_seqs ? 8 : 16; }
+
+struct Layout {
+  int rt;
+  int64_t tiles, parts;
+  uint64_t ml_at, part_at, bytes;
+};
+Layout layout_of(int n, int n_seqs, int nh, int nkv, int hs) {
+  Layout s;
+  const int group = nh / nkv;
+  s.rt = rows_of_tile(n, n_seqs, group);
+  s.tiles = ((int64_t)n * group + s.rt - 1) / s.rt + (n < n_seqs ? n : n_seqs);
+  s.parts = s.tiles + (MOST_BLOCKS + nkv - 1) / nkv;
+  const auto up = [](uint64_t x) { return (x + 255) / 256 * 256; };
+  s.ml_at = up((s.tiles + 1) * sizeof(int4));
+  s.part_at = s.ml_at + up(s.parts * nkv * s.rt * sizeof(float2));
+  s.bytes = s.part_at + up(s.parts * nkv * s.rt * (uint64_t)hs * sizeof(float));
+  return s;
+}
+
+template <int HSEG, int RT, bool HALF>
+int launch_attention8(const Args &a, int blocks_x, cudaStream_t stream) {
+  using S = Shape<HSEG, RT, HALF>;
+  auto kernel = cache8_attention_kernel<HSEG, RT, HALF>;
+  B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename S::Smem)));
+  const int most = 148 * S::MINB / a.nkv;
+  launch(kernel, dim3(most < 1 ? 1 : most < blocks_x ? most : blocks_x, a.nkv), dim3(THREADS), sizeof(typename S::Smem),
+         stream, a);
+  B200_LAUNCHED("cache8_attention");
+  return 0;
+}
+
+int check_sizes(const char *what, int n, int n_seqs, int nh, int nkv, int hs) {
+  const std::string name(what);
+  if (n < 0 || n_seqs < 1 || n_seqs > 65536) return fail(B200FWD_EINVAL, name + ": 1 to 65536 requests, no fewer than 0 tokens");
+  if (nkv < 1 || nh < nkv || nh % nkv || nkv > 1024)
+    return fail(B200FWD_EINVAL, name + ": the heads are a multiple of the kv heads, 1 to 1024 of them");
+  if (hs < 16 || hs > 256 || hs % 16)
+    return fail(B200FWD_EINVAL, name + ": the head size is a multiple of 16, at most 256");
+  if ((int64_t)n * nh > INT32_MAX / 2) return fail(B200FWD_EINVAL, name + ": more rows (tokens times heads) than 2^30");
+  return 0;
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200k_cache8_attention_scratch(int32_t n, int32_t n_seqs, int32_t nh, int32_t nkv, int32_t hs,
+                                              int32_t half, uint64_t *bytes) {
+  try {
+    (void)half;
+    if (!bytes) return fail(B200FWD_EINVAL, "cache8_attention_scratch: null pointer");
+    const int rc = check_sizes("cache8_attention_scratch", n, n_seqs, nh, nkv, hs);
+    if (rc) return rc;
+    *bytes = layout_of(n, n_seqs, nh, nkv, hs).bytes;
+    return 0;
+  } catch (...) {
+    return fail(B200FWD_EINVAL, "cache8_attention_scratch: exception");
+  }
+}
+
+extern "C" int b200k_cache8_attention(void *out, const void *q, const int8_t *kc, const float *ks, const int8_t *vc,
+                                      const float *vs, const int32_t *tables, const int32_t *starts,
+                                      const int32_t *lengths, int32_t n, int32_t n_seqs, int32_t table_width,
+                                      int32_t blocks, int32_t block, int32_t nh, int32_t nkv, int32_t hs,
+                                      int64_t q_stride, int64_t out_stride, int32_t half, void *scratch,
+                                      b200fwd_stream stream) {
+  try {
+    const char *what = "cache8_attention";
+    int rc = check_sizes(what, n, n_seqs, nh, nkv, hs);
+    if (!rc) rc = check_cache8(what, kc, ks, vc, vs, blocks, block, nkv, hs);
+    if (rc) return rc;
+    if (n == 0) return 0;
+    if (!out || !q || !tables || !starts || !lengths || !scratch)
+      return fail(B200FWD_EINVAL, "cache8_attention: null pointer");
+    if (table_width < 1 || (int64_t)table_width * block > INT32_MAX / 2)
+      return fail(B200FWD_EINVAL, "cache8_attention: a table row of 1 block at least and 2^30 positions at most");
+    const int64_t row = (int64_t)nh * hs, to = half ? 8 : 4;
+    if (q_stride < row || out_stride < row || q_stride % to || out_stride % to ||
+        reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16)
+      return fail(B200FWD_EINVAL, "cache8_attention: rows of q and out of nh * hs values at least, on 16 bytes");
+    if (reinterpret_cast<uintptr_t>(scratch) % 256)
+      return fail(B200FWD_EINVAL, "cache8_attention: scratch must be 256-byte aligned");
+    const Layout s = layout_of(n, n_seqs, nh, nkv, hs);
+    uint8_t *base = reinterpret_cast<uint8_t *>(scratch);
+    Args a = {out, q, kc, vc, ks, vs, tables, starts, lengths, reinterpret_cast<int4 *>(base) + 1,
+              reinterpret_cast<float2 *>(base + s.ml_at), reinterpret_cast<float *>(base + s.part_at), q_stride,
+              out_stride, n, n_seqs, table_width, blocks, block, nkv, hs, nh / nkv, 8, s.tiles,
+              1.4426950408889634f / sqrtf((float)hs)};
+    const cudaStream_t st = as_stream(stream);
+    const int hseg = (hs + 63) / 64, blocks_x = (MOST_BLOCKS + nkv - 1) / nkv;
+    using Launch = int (*)(const Args &, int, cudaStream_t);
+    static const Launch table[4][2][2] = {
+        {{launch_attention8<1, 8, false>, launch_attention8<1, 8, true>}, {launch_attention8<1, 16, false>, launch_attention8<1, 16, true>}},
+        {{launch_attention8<2, 8, false>, launch_attention8<2, 8, true>}, {launch_attention8<2, 16, false>, launch_attention8<2, 16, true>}},
+        {{launch_attention8<3, 8, false>, launch_attention8<3, 8, true>}, {launch_attention8<3, 16, false>, launch_attention8<3, 16, true>}},
+        {{launch_attention8<4, 8, false>, launch_attention8<4, 8, true>}, {launch_attention8<4, 16, false>, launch_attention8<4, 16, true>}}};
+    rc = table[hseg - 1][s.rt == 16][half ? 1 : 0](a, blocks_x, st);
+    if (rc) return rc;
+    // a row a thread block where there are few rows (the joining of a long request's many spans is what takes time
+    // then), else a tile
+    const dim3 grid((unsigned)s.tiles, nkv, s.tiles * nkv <= 1024 ? s.rt : 1);
+    auto combine = s.rt == 8 ? (half ? cache8_combine_kernel<8, true> : cache8_combine_kernel<8, false>)
+                             : (half ? cache8_combine_kernel<16, true> : cache8_combine_kernel<16, false>);
+    launch(combine, grid, dim3(CW * 32), 0, st, a);
+    B200_LAUNCHED("cache8_combine");
+    return 0;
+  } catch (...) {
+    return fail(B200FWD_EINVAL, "cache8_attention: exception");
+  }
+}
