@@ -341,7 +341,7 @@ int b200k_cache8_load(void *k, void *v, const int8_t *kc, const float *ks, const
  * sees no position (fewer positions than tokens) is 0; a row that sees a position whose table entry is no block, or
  * past its table row, is NaN. Rows that belong to no request are left as they were; starts that do not ascend within
  * 0..n leave out unwritten. Not to the bit like b200k_attention, but within float32's rounding (half: float16's) of the
- * exact result for the stored values; the same call gives the same bits. Up to 65536 requests, n * nh up to 2^30,
+ * exact result for the stored values; the same call gives the same bits. Up to 65536 requests, n up to 2^25 and n * nh to 2^30,
  * table_width * block up to 2^30. scratch: b200k_cache8_attention_scratch() bytes of device memory, 256-byte aligned,
  * nothing zeroed; calls that overlap on the GPU need one each. */
 int b200k_cache8_attention(void *out, const void *q, const int8_t *kc, const float *ks, const int8_t *vc,

@@ -18,58 +18,29 @@
 // joins in the order of the spans: results don't depend on timing.
 // Loads: each lane copies the bytes that it will multiply itself (cp.async into a ring of its own, so no thread waits
 // for another), stages deep enough to cover HBM's latency.
-#include <cuda_fp16.h>
-
-#include <cstdint>
 #include <string>
 
 #include "cache8.h"
-#include "common.h"
+#include "cache8_attention.cuh"
 
 namespace b200 {
+using namespace cache8;
 namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int UNIT = 16;          // positions of a unit: one operand tile, within one block of the cache
 constexpr int RING = 16384;       // bytes of a warp's ring
-constexpr float RESCALE = 8.0f;   // log2 of how far a weight may rise above 1 before M moves
 constexpr int MOST_BLOCKS = 148 * 3;  // thread blocks of a grid (resident at once)
 
-struct Args {
-  void *out;
-  const void *q;
-  const int8_t *kc, *vc;
-  const float *ks, *vs;
-  const int32_t *tables, *starts, *lengths;
-  int4 *meta;       // [tiles] {first span, spans, request, row tile}; meta[-1].x: the tiles
-  float2 *part_ml;  // [span + tile][kv head][RT] {M, l}
-  float *part;      // [span + tile][kv head][RT][hs]
-  int64_t q_stride, out_stride;
-  int n, n_seqs, width, blocks, block, nkv, hs, group, min_units;
-  int64_t most_tiles;
-  float scale;      // log2(e) / sqrt(hs)
-};
-
-// request i of the call: its first row, its rows, and its positions (all of them, the new ones included)
-struct Request {
-  int first, fresh, length;
-};
-__device__ __forceinline__ Request request_of(const Args &a, int i) {
-  const int s0 = min(max(a.starts[i], 0), a.n), s1 = min(max(a.starts[i + 1], s0), a.n);
-  return {s0, s1 - s0, max(a.lengths[i], 0)};
-}
 template <int RT>
 __device__ __forceinline__ int tiles_of(const Args &a, const Request &r) {
-  return (r.fresh * a.group + RT - 1) / RT;
+  const int rows = r.fresh * a.group;
+  return rows > a.rows_most ? 0 : (rows + RT - 1) / RT;
 }
 // its units: the positions that its table has room for, one unit at least (a row that sees nothing is written too)
 __device__ __forceinline__ int units_of(const Args &a, const Request &r) {
   return max(1, (min(r.length, a.width * a.block) + UNIT - 1) / UNIT);
 }
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
 // BYTES (4, 8 or 16) to shared memory, zeros where !on (then nothing is read)
 template <int BYTES>
 __device__ __forceinline__ void copy(uint32_t dst, const void *src, bool on) {
@@ -85,25 +56,6 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-__device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2 *>(&u)); }
-// two of a word's bytes (already + 128) as float16 integers: 1024 + b is a float16 whose low byte is b
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t widen(uint32_t biased) {
-  uint32_t d;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(biased), "r"(0x64646464u), "n"(SEL));
-  const __half2 v = __hsub2(*reinterpret_cast<__half2 *>(&d), __half2half2(__ushort_as_half(0x6480)));  // less 1152
-  return *reinterpret_cast<const uint32_t *>(&v);
-}
 __device__ __forceinline__ uint32_t interleave_lo(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5140); }
 __device__ __forceinline__ uint32_t interleave_hi(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7362); }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -178,22 +130,22 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
   const int h = blockIdx.y;
 
   // ---- this block's span of the units
-  int64_t total = 0, all_tiles = 0;
+  int64_t total = 0, fresh = 0;
   for (int i = tid; i < a.n_seqs; i += THREADS) {
     const Request r = request_of(a, i);
-    all_tiles += tiles_of<RT>(a, r);
+    fresh += r.fresh;
     total += (int64_t)tiles_of<RT>(a, r) * units_of(a, r);
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
     total += __shfl_xor_sync(0xffffffffu, total, d);
-    all_tiles += __shfl_xor_sync(0xffffffffu, all_tiles, d);
+    fresh += __shfl_xor_sync(0xffffffffu, fresh, d);
   }
-  if (lane == 0) sm.part[0][warp] = total, sm.part[1][warp] = all_tiles;
+  if (lane == 0) sm.part[0][warp] = total, sm.part[1][warp] = fresh;
   __syncthreads();
   total = sm.part[0][0] + sm.part[0][1] + sm.part[0][2] + sm.part[0][3];
-  all_tiles = sm.part[1][0] + sm.part[1][1] + sm.part[1][2] + sm.part[1][3];
-  if (all_tiles > a.most_tiles) total = 0;  // starts that don't ascend: rows of several requests, nothing is written
+  fresh = sm.part[1][0] + sm.part[1][1] + sm.part[1][2] + sm.part[1][3];
+  if (fresh > a.n) total = 0;  // starts that don't ascend: rows of several requests, nothing is written
   const int64_t span = max((int64_t)a.min_units, (total + gridDim.x - 1) / gridDim.x);
   int64_t at = span * blockIdx.x;
   const int64_t end = min(at + span, total);
@@ -227,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
     if (blockIdx.x == 0 && h == 0 && tid == 0) a.meta[-1] = make_int4((int)carry[1], 0, 0, 0);
   }
 
-  const uint32_t ring = smem_u32(sm.ring[warp]);
+  const uint32_t ring = smem_addr(sm.ring[warp]);
   uint8_t *ring_p = sm.ring[warp];
   while (at < end) {
     const Request r = request_of(a, req);
@@ -363,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
         // a table entry that is no block of the pool: NaN scales, so every row that sees it comes out NaN
         if (lane < 2) {
           float *dst_s = &sm.sc[warp][slot][lane];
-          if (ok) copy<4>(smem_u32(dst_s), (lane ? a.vs : a.ks) + ph, true);
+          if (ok) copy<4>(smem_addr(dst_s), (lane ? a.vs : a.ks) + ph, true);
           else *dst_s = __uint_as_float(0x7fffffffu);
         }
       }
@@ -411,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
         }
         // ---- weights. A value scale below 2^-100 counts as 2^-100 (a block of zeros has scale 0): what it weighs
         // is below any other block's last place
-        const float vs = !(vscale < 7.888609e-31f) ? vscale : 7.888609e-31f;
+        const float vs = !(vscale < LEAST) ? vscale : LEAST;
         const float lg = __log2f(vs), inv = __fdiv_rn(1.0f, vs);
         const bool masked = u * UNIT + UNIT - 1 > first;
         bool up = false;
@@ -674,7 +626,8 @@ int check_sizes(const char *what, int n, int n_seqs, int nh, int nkv, int hs) {
     return fail(B200FWD_EINVAL, name + ": the heads are a multiple of the kv heads, 1 to 1024 of them");
   if (hs < 16 || hs > 256 || hs % 16)
     return fail(B200FWD_EINVAL, name + ": the head size is a multiple of 16, at most 256");
-  if ((int64_t)n * nh > INT32_MAX / 2) return fail(B200FWD_EINVAL, name + ": more rows (tokens times heads) than 2^30");
+  if ((int64_t)n * nh > INT32_MAX / 2 || n > 1 << 25)
+    return fail(B200FWD_EINVAL, name + ": more rows (tokens times heads) than 2^30, or more tokens than 2^25");
   return 0;
 }
 
@@ -721,9 +674,13 @@ extern "C" int b200k_cache8_attention(void *out, const void *q, const int8_t *kc
       return fail(B200FWD_EINVAL, "cache8_attention: scratch must be 256-byte aligned");
     const Layout s = layout_of(n, n_seqs, nh, nkv, hs);
     uint8_t *base = reinterpret_cast<uint8_t *>(scratch);
+    // blocks of tokens go to the tensor cores; where there is no more than a token a request on average, any request is
+    // taken here, and one kernel less launched
+    const bool prompts = n > n_seqs && prompts_fit(hs);
     Args a = {out, q, kc, vc, ks, vs, tables, starts, lengths, reinterpret_cast<int4 *>(base) + 1,
               reinterpret_cast<float2 *>(base + s.ml_at), reinterpret_cast<float *>(base + s.part_at), q_stride,
-              out_stride, n, n_seqs, table_width, blocks, block, nkv, hs, nh / nkv, 8, s.tiles,
+              out_stride, n, n_seqs, table_width, blocks, block, nkv, hs, nh / nkv, 8,
+              prompts ? ROWS_FEW : INT32_MAX,
               1.4426950408889634f / sqrtf((float)hs)};
     const cudaStream_t st = as_stream(stream);
     const int hseg = (hs + 63) / 64, blocks_x = (MOST_BLOCKS + nkv - 1) / nkv;
@@ -734,6 +691,7 @@ extern "C" int b200k_cache8_attention(void *out, const void *q, const int8_t *kc
         {{launch_attention8<3, 8, false>, launch_attention8<3, 8, true>}, {launch_attention8<3, 16, false>, launch_attention8<3, 16, true>}},
         {{launch_attention8<4, 8, false>, launch_attention8<4, 8, true>}, {launch_attention8<4, 16, false>, launch_attention8<4, 16, true>}}};
     rc = table[hseg - 1][s.rt == 16][half ? 1 : 0](a, blocks_x, st);
+    if (!rc && prompts) rc = launch_attention8_prompts(a, half, st);
     if (rc) return rc;
     // a row a thread block where there are few rows (the joining of a long request's many spans is what takes time
     // then), else a tile

@@ -73,8 +73,9 @@ def store(cache, scales, x, slots, block):
         i += m
 
 
-def attention(q, kc, ks, vc, vs, tables, starts, lengths, block, group):
-    """(out, bound) of q [n][heads][size] in float64; bound: what an element may be off in float32 arithmetic (see there)."""
+def attention(q, kc, ks, vc, vs, tables, starts, lengths, block, group, half=False):
+    """(out, bound) of q [n][heads][size] in float64; bound: what an element may be off in float32 arithmetic (see there),
+    with float16 queries and outputs where half."""
     n, heads, size = q.shape
     out, bound = np.full(q.shape, np.nan), np.zeros(q.shape)
     eps = 2.0 ** -23
@@ -113,6 +114,10 @@ def attention(q, kc, ks, vc, vs, tables, starts, lengths, block, group):
                 units = last // 16 + 1
                 bound[t, h] = (p @ np.abs(v[:last + 1])) * (2 * weight + (4 * units + 32) * eps)
                 integers = np.abs(vc[page, kv].astype(np.float64)).reshape(-1, size)[:last + 1]
+                if half:
+                    # half a step of float16, 2^-11 of a value at most, once for a weight (the prompts' kernel keeps
+                    # float16 requests' weights in one part) and once for the output
+                    bound[t, h] += (p @ np.abs(v[:last + 1])) * 2.0 ** -11 + np.abs(out[t, h]) * 2.0 ** -11 + 2.0 ** -25
                 bound[t, h] += 2.0 ** -25 * integers.sum(0) * (p * np.repeat(vs[page, kv], block)[:last + 1]).max()
     return out, bound
 

@@ -330,9 +330,7 @@ class Case:
 
     def check(self, got):
         want, bound = plain.attention(self.q64, self.kc, self.ks, self.vc, self.vs, self.tables, self.starts, self.lengths,
-                                      self.block, self.heads // self.nkv)
-        if self.half:
-            bound = bound + np.abs(want) * 2.0 ** -11 + 2.0 ** -25  # the output's own rounding
+                                      self.block, self.heads // self.nkv, self.half)
         off = np.abs(got - want)
         assert (off <= bound).all(), (np.argwhere(~(off <= bound))[:5], np.nanmax(off / bound))
 
@@ -405,8 +403,7 @@ def test_attention_bad_pages(fresh, half):
     blind[c.starts[1] + max(0, fresh - 8):c.starts[2]] = True
     blind[c.starts[2]:] = True
     assert np.isnan(got[blind]).all()
-    want, bound = plain.attention(c.q64, c.kc, c.ks, c.vc, c.vs, c.tables, c.starts, c.lengths, c.block, 2)
-    bound = bound + (np.abs(want) * 2.0 ** -11 + 2.0 ** -25 if half else 0)
+    want, bound = plain.attention(c.q64, c.kc, c.ks, c.vc, c.vs, c.tables, c.starts, c.lengths, c.block, 2, half)
     assert (np.abs(got - want) <= bound)[~blind].all()
 
 
@@ -583,9 +580,7 @@ class Server:
         for got, want in ((self.kc, kc), (self.ks, ks), (self.vc, vc), (self.vs, vs)):
             assert np.array_equal(host(got), want, equal_nan=want.dtype == np.float32)
         want, bound = plain.attention(q.reshape(self.n, self.heads, self.hs), kc, ks, vc, vs, t.tables, starts, t.lengths,
-                                      self.block, self.heads // self.nkv)
-        if self.half:
-            bound = bound + np.abs(want) * 2.0 ** -11 + 2.0 ** -25
+                                      self.block, self.heads // self.nkv, self.half)
         got = floats(self.out, self.half).reshape(self.n, self.heads, self.hs)
         live = slice(0, int(starts[-1]))
         assert (np.abs(got[live] - want[live]) <= bound[live]).all()
