@@ -2,20 +2,24 @@
 // query rows a kv head), on the 5th-generation tensor cores: the numbers of cache8_attention.cu, whose comment has the
 // mathematics (float16 pairs for float32, scales outside the products, weights relative to the largest term).
 //
-// A thread block takes two neighbouring tiles of 128 rows of one request and kv head (row x: query head x % group of the
-// request's token x / group, so the heads that share a kv head share its keys) and walks their positions in steps of 64.
-// 512 threads:
-//   warps 0..3 bring the cache: int8 keys and values by 16-byte loads one step ahead, widened to float16 (exact) into
-//     shared memory in the tensor cores' 128-byte swizzled layout, for both tiles at once; a step's four units'
-//     scales beside them. Positions are rows of both: for K Q^T they run along N, for P V along K, and the values'
-//     operand is described as major along the head, so nothing is transposed;
-//   warps 4..7 and 8..11 the softmax of each tile, a thread a row (TMEM lane): scores from TMEM, weights as float16
-//     (float32 queries: a high and a low part, in the two halves of the scores' columns) back over them;
-//   warp 12 issues the products: S = Q K^T (M 128, N 64; float32: once for each part of Q) into one of a tile's two
-//     score buffers, O += P V (M 128, N head size; float32: once for each part of P) with P read from TMEM.
-// Bound by the tensor cores and the exponentials about alike (float16 queries, heads of 128: a step of two tiles is
-// 1024 cycles of each), with the widening under both; float32 queries double the products.
-// TMEM (512 columns): tile t's score buffers at 128 t + {0, 64}, its O at 256 + 128 t (64 t at heads of 64).
+// A thread block takes 256 (float16) or 128 (float32) rows of one request and kv head, in tiles of 128 (row x: query head
+// x % group of the request's token x / group, so the heads that share a kv head share its keys), and walks their
+// positions in steps of 64. 640 threads:
+//   warps 0..7 bring the cache: int8 keys and values by 16-byte loads one step ahead, widened to float16 (exact) into
+//     shared memory in the tensor cores' 128-byte swizzled layout; a step's four units' scales beside them. Positions
+//     are rows of both: for K Q^T they run along N, for P V along K, and the values' operand is described as major along
+//     the head, so nothing is transposed;
+//   warps 8..11 the softmax of the first tile, a thread a row (TMEM lane): scores from TMEM, weights as float16 (float32
+//     queries: a high and a low part, in the two halves of the scores' columns) back over them;
+//   warps 12..15, float16: the softmax of the second tile. The products add up in TMEM, which is rescaled there when a
+//     row's maximum moves. float32: they add up each step's product in registers. (The tensor cores' float32 sums are
+//     cut off rather than rounded: over 2048 positions that came to 2.5e-6 of the outputs, of one step it is nothing.)
+//   warps 16..19 issue the products, two a tile: S = Q K^T (M 128, N 64; float32: once for each part of Q) and O = P V
+//     (M 128, N head size; float32: once for each part of P) with P read from TMEM.
+// Bound by the tensor cores and, close behind, by instructions issued (float16, heads of 128: a step is 1024 cycles of
+// products, as many of exponentials, and about as many issue slots, a third of them for widening).
+// TMEM (512 columns), float16: tile t's two score buffers at 128 t + {0, 64}, its O at 256 + t * head size; float32: three
+// score buffers at {0, 64, 128}, two of O at 192 + {0, 1} * head size.
 // Every wait is bounded: past it the kernel sets the scratch's error word and runs to its end.
 #include <string>
 
@@ -28,31 +32,54 @@ namespace {
 
 using namespace tc;
 
-constexpr int QT = 128, KT = 64, THREADS = 512, KU = KT / UNIT;
+constexpr int QT = 128, KT = 64, THREADS = 640, KU = KT / UNIT;
+constexpr int BRINGERS = 256;  // threads that bring the cache
+constexpr int SORTED = 64;     // requests that are taken in order of their lengths
 
 template <int HP, bool HALF>
 struct Tc {
-  static constexpr int CHUNKS = HP / 64;              // 128-byte columns of 64 float16
-  static constexpr int PARTS = HALF ? 1 : 2;          // of a float32 number
-  static constexpr int STAGES = HP == 128 && !HALF ? 3 : 4;
+  static constexpr int TILES = HALF ? 2 : 1;
+  static constexpr int CHUNKS = HP / 64;  // 128-byte columns of 64 float16
+  static constexpr int PARTS = HALF ? 1 : 2;
+  static constexpr int STAGES = 4;
+  static constexpr int SBUF = HALF ? 2 : 3;  // score buffers of a tile
   struct Smem {
-    alignas(1024) uint8_t q[2][PARTS][CHUNKS][QT * 128];
+    alignas(1024) uint8_t q[TILES][PARTS][CHUNKS][QT * 128];
     alignas(1024) uint8_t k[STAGES][CHUNKS][KT * 128];
     alignas(1024) uint8_t v[STAGES][CHUNKS][KT * 128];
     alignas(16) float4 sc[STAGES][KU];  // a unit's {key scale * log2(e) / sqrt(hs), log2(value scale), 1 / value scale}
+    float by[4][QT], l[QT];             // float32: what the rows' sums so far are scaled by at a step; the row sums
     uint64_t q_full, kv_full[STAGES], kv_empty[STAGES];
-    uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], mma_done;  // [tile][buffer]
+    uint64_t s_full[TILES][SBUF], p_full[TILES][SBUF], pv_done[TILES][SBUF], o_free[2], by_full[4], l_full, mma_done;
     uint32_t tmem_base;
     int part[2][THREADS / 32], found[2];
+    int2 of[SORTED];                    // the requests' positions and groups of tiles
   };
 };
 
-// A from TMEM (float16 pairs along K), B from shared memory
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int acc) {
+// The thread of a converged warp that issues its products. (elect.sync rather than a lane's number: the products' operands
+// go through the warp's uniform registers, and what the compiler makes of a branch on the lane, predicates among it, left
+// other lanes' values in them; with a predicate of one's own on every product a product took 100 cycles to issue, 66 so.)
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p;
+}
+// D (+)= A B, A from shared memory or from TMEM (float16 pairs along K), B from shared memory
+template <bool ADD>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "n"(ADD ? 1 : 0)
+      : "memory");
+}
+template <bool ADD>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "r"(a), "l"(b), "r"(idesc), "n"(ADD ? 1 : 0)
       : "memory");
 }
 // The values: 128-byte rows of 64 head values, a row a position, swizzled. Major along the head (N): the next 64 of the
@@ -115,10 +142,12 @@ __device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uin
 __device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
 // One step of this thread's row: 64 scores from tS, their weights over them. EDGE: some of the tile's rows don't see all
-// of the step (pos: this row's last position, first: the step's first). m, l: the row's running maximum and sum.
-template <int HP, bool HALF, bool EDGE>
-__device__ __forceinline__ void softmax_step(uint32_t tS, uint32_t tO, const float4 *sc, float qf, int pos, int first,
-                                             int j, float &m, float &l, uint64_t (*pv_done)[2], int *error) {
+// of the step; limit: the last position that this row sees, from the step's first. m, l: the row's running maximum and
+// sum. settle(top): called by the whole warp where some row's maximum moves, to `top`; what it returns the sum is
+// scaled by.
+template <int HP, bool HALF, bool EDGE, typename Settle>
+__device__ __forceinline__ void softmax_step(uint32_t tS, const float4 *sc, float qf, int limit, float &m, float &l,
+                                             Settle &&settle) {
   float x[KT];
   ld32(tS, x);
   ld32(tS + 32, x + 32);
@@ -127,6 +156,8 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, uint32_t tO, const flo
   for (int u = 0; u < KU; u++) {
     const float4 s = sc[u];
     c[u] = s.x * qf, lg[u] = s.y, inv[u] = s.z;
+    // (a unit that the row does not see may have any scales, NaN too)
+    if (EDGE && u * UNIT > limit) c[u] = 1.0f, lg[u] = 0.0f, inv[u] = 0.0f;
   }
   tmem_wait_ld();
   float most = -INFINITY;
@@ -135,7 +166,7 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, uint32_t tO, const flo
     if (EDGE) {
 #pragma unroll
       for (int i = 0; i < UNIT; i++)
-        if (first + u * UNIT + i > pos) x[u * UNIT + i] = -INFINITY;
+        if (u * UNIT + i > limit) x[u * UNIT + i] = -INFINITY;
     }
     float top = x[u * UNIT];
 #pragma unroll
@@ -143,26 +174,12 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, uint32_t tO, const flo
     top = fmaxf(top, x[u * UNIT + UNIT - 1]);
     most = fmaxf(most, __fmaf_rn(top, c[u], lg[u]));
   }
-  if (j == 0) {
-    m = most;
-  } else if (__any_sync(0xffffffffu, most > m + RESCALE)) {
-    // O holds the steps so far: once the last P V is done, it and the sum go to the new maxima (the whole warp's rows:
-    // TMEM is read and written by whole warps)
-    mbar_wait(&(*pv_done)[(j - 1) & 1], ((j - 1) >> 1) & 1, error, 109);
-    __syncwarp();
-    fence_after();
-    const float top = fmaxf(m, most), f = m == top ? 1.0f : ex2(m - top);
-#pragma unroll
-    for (int ch = 0; ch < HP / 32; ch++) {
-      float o[32];
-      ld32(tO + ch * 32, o);
-      tmem_wait_ld();
-#pragma unroll
-      for (int i = 0; i < 32; i++) o[i] *= f;
-      st32(tO + ch * 32, o);
-    }
-    l *= f;
+  if (__any_sync(0xffffffffu, most > m + RESCALE)) {
+    const float top = fmaxf(m, most);
+    l *= settle(m == top ? 1.0f : ex2(m - top));
     m = top;
+  } else {
+    settle(-1.0f);
   }
   const float from = m == -INFINITY ? 0.0f : m;
 #pragma unroll
@@ -173,11 +190,7 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, uint32_t tO, const flo
 #pragma unroll
     for (int i = 0; i < UNIT; i += 2) {
       const uint64_t e = fma_2(f2(x[u * UNIT + i], x[u * UNIT + i + 1]), c2, a2);
-      float w0 = ex2(lo_of(e)), w1 = ex2(hi_of(e));
-      if (EDGE) {
-        if (first + u * UNIT + i > pos) w0 = 0.0f;
-        if (first + u * UNIT + i + 1 > pos) w1 = 0.0f;
-      }
+      const float w0 = ex2(lo_of(e)), w1 = ex2(hi_of(e));
       sum = add_2(sum, f2(w0, w1));
       hi[i / 2] = pack(w0, w1);
       if (!HALF) {
@@ -185,8 +198,7 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, uint32_t tO, const flo
         lo[i / 2] = pack(w0 - b.x, w1 - b.y);
       }
     }
-    // (a unit that the row does not see: 0 times a scale that may be NaN)
-    l = __fmaf_rn(lo_of(sum) + hi_of(sum), !EDGE || first + u * UNIT <= pos ? inv[u] : 0.0f, l);
+    l = __fmaf_rn(lo_of(sum) + hi_of(sum), inv[u], l);
     st8(tS + 8 * u, hi);
     if (!HALF) st8(tS + 32 + 8 * u, lo);
   }
@@ -196,25 +208,29 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, uint32_t tO, const flo
 template <int HP, bool HALF>
 __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const Args a) {
   using S = Tc<HP, HALF>;
-  constexpr int STAGES = S::STAGES, PARTS = S::PARTS;
+  constexpr int STAGES = S::STAGES, PARTS = S::PARTS, TILES = S::TILES, SBUF = S::SBUF;
   extern __shared__ uint8_t raw[];
   typename S::Smem &s = *reinterpret_cast<typename S::Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   pdl_begin();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // (a tile group's heads side by side)
+  const int h = blockIdx.x % a.nkv, index = blockIdx.x / a.nkv;
   int *error = &a.meta[-1].y;
 
-  // ---- which request's which pair of tiles
+  // ---- which request's which group of TILES tiles: a request's last rows, which see the most positions, first, and up to
+  // SORTED requests the longest first (a block's time is its positions'; what starts last should be short)
   int total = 0, fresh = 0;
   if (tid == 0) s.found[0] = -1;
   for (int base = 0; base < a.n_seqs; base += THREADS) {
     const int i = base + tid;
-    int pairs = 0, own = 0;
+    int groups = 0, own = 0;
     if (i < a.n_seqs) {
       const Request r = request_of(a, i);
       own = r.fresh;
-      pairs = r.fresh * a.group > a.rows_most ? (r.fresh * a.group + 2 * QT - 1) / (2 * QT) : 0;
+      groups = r.fresh * a.group > a.rows_most ? (r.fresh * a.group + TILES * QT - 1) / (TILES * QT) : 0;
+      if (a.n_seqs <= SORTED) s.of[tid] = make_int2(r.length, groups);
     }
-    int upto = pairs;
+    int upto = groups;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int o = __shfl_up_sync(0xffffffffu, upto, d);
@@ -230,42 +246,54 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       total += s.part[0][w];
       fresh = min(fresh + s.part[1][w], a.n + 1);
     }
-    const int x = (int)blockIdx.x - (before + upto - pairs);
-    // the request's last pair, which sees the most positions, first
-    if (x >= 0 && x < pairs) s.found[0] = i, s.found[1] = pairs - 1 - x;
+    before += upto - groups;
+    if (a.n_seqs <= SORTED && i < a.n_seqs) {
+      before = 0;
+      const int length = s.of[tid].x;
+      for (int k = 0; k < a.n_seqs; k++) {
+        const int2 o = s.of[k];
+        if (o.x > length || (o.x == length && k < i)) before += o.y;
+      }
+    }
+    const int x = index - before;
+    if (x >= 0 && x < groups) s.found[0] = i, s.found[1] = groups - 1 - x;
   }
   if (fresh > a.n) return;  // starts that don't ascend
   __syncthreads();
-  const int req = s.found[0], pair = s.found[1];
+  const int req = s.found[0];
   if (req < 0) return;
   const Request r = request_of(a, req);
-  const int rows = r.fresh * a.group, cap = a.width * a.block, row0 = pair * 2 * QT;
+  const int rows = r.fresh * a.group, cap = a.width * a.block, row0 = s.found[1] * TILES * QT;
   // steps of each tile: up to its last row's position (and within the table's row)
-  int steps[2];
+  int steps[2] = {0, 0}, most_steps = 0;
 #pragma unroll
-  for (int t = 0; t < 2; t++) {
+  for (int t = 0; t < TILES; t++) {
     const int x = min(rows, row0 + (t + 1) * QT) - 1;  // the tile's last row
     const int seen = x < row0 + t * QT ? 0 : min(r.length - r.fresh + x / a.group + 1, cap);
     steps[t] = max(0, (seen + KT - 1) / KT);
+    most_steps = max(most_steps, steps[t]);
   }
-  const int most_steps = max(steps[0], steps[1]);
 
   if (tid == 0) {
-    mbar_init(&s.q_full, 2 * QT);
+    mbar_init(&s.q_full, TILES * QT);
     for (int i = 0; i < STAGES; i++) {
-      mbar_init(&s.kv_full[i], QT);
-      mbar_init(&s.kv_empty[i], 1);
+      mbar_init(&s.kv_full[i], BRINGERS);
+      mbar_init(&s.kv_empty[i], TILES);
     }
-    for (int t = 0; t < 2; t++)
-      for (int u = 0; u < 2; u++) {
+    for (int t = 0; t < TILES; t++) {
+      for (int u = 0; u < SBUF; u++) {
         mbar_init(&s.s_full[t][u], 1);
         mbar_init(&s.p_full[t][u], 4);
         mbar_init(&s.pv_done[t][u], 1);
       }
-    mbar_init(&s.mma_done, 1);
+    }
+    for (int u = 0; u < 2; u++) mbar_init(&s.o_free[u], 4);
+    for (int u = 0; u < 4; u++) mbar_init(&s.by_full[u], 4);
+    mbar_init(&s.l_full, 4);
+    mbar_init(&s.mma_done, 2 * TILES);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem_base)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -273,24 +301,57 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
   __syncthreads();
   fence_after();
   const uint32_t tmem = s.tmem_base;
-  auto tS = [&](int t, int u) { return tmem + (uint32_t)(t * 2 * KT + u * KT); };
-  auto tO = [&](int t) { return tmem + (uint32_t)(4 * KT + t * HP); };
+  auto tS = [&](int t, int u) { return tmem + (uint32_t)((t * SBUF + u) * KT); };
+  auto tO = [&](int t) { return tmem + (uint32_t)((TILES * SBUF) * KT + t * HP); };  // float32: t the buffer
 
-  // (the launch's 512 x 128 registers: 128 x (96 + 176 + 176 + 56) = 512 x 126)
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+  // this thread's row of its tile (softmax and summing threads; TMEM lane y)
+  const int y = tid & 127, t_own = HALF && warp >= 12 ? 1 : 0, x_own = row0 + t_own * QT + y;
+  const bool on = x_own < rows;
+  const int token = on ? x_own / a.group : 0, head = h * a.group + (on ? x_own % a.group : 0);
+  const int pos = on ? r.length - r.fresh + token : -1;
+  const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+  // 8 values z of the output row from value d on
+  auto put = [&](int d, const float (&z)[8]) {
+    const int64_t off = (int64_t)(r.first + token) * a.out_stride + (int64_t)head * a.hs + d;
+    if (HALF) {
+      *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(a.out) + off) =
+          make_uint4(pack(z[0], z[1]), pack(z[2], z[3]), pack(z[4], z[5]), pack(z[6], z[7]));
+    } else {
+      float4 *dst = reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + off);
+      dst[0] = make_float4(z[0], z[1], z[2], z[3]);
+      dst[1] = make_float4(z[4], z[5], z[6], z[7]);
+    }
+  };
+  // 1 / the row sum; a row that sees nothing is 0, one past its table's row (or after a wait that gave up) NaN
+  auto inverse = [&](float l, bool ok) {
+    return !ok || pos >= cap ? __uint_as_float(0x7fffffffu) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+  };
+
+  // (the launch's 640 x 96 registers: 128 x (64 + 64 + 144 + 168 + 40) = 640 x 96)
+  if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // ---- the cache: thread tid brings 16 bytes of rows tid / CH + i * PER (CH pieces a row) of keys and of values
-    constexpr int CH = HP / 16, PER = QT / CH, R = KT / PER;
+    constexpr int CH = HP / 16, PER = BRINGERS / CH, R = KT / PER;
     const int32_t *table = a.tables + (int64_t)req * a.width;
     const int piece = tid % CH, brow = tid / CH;
     const bool in_head = piece * 16 < a.hs;
-    const int last_unit = min(cap, r.length) / UNIT;  // (units past it are no row's to see, or belong to NaN rows)
-    auto page_of = [&](int u) { return u <= last_unit && u * UNIT < cap ? table[u * UNIT / a.block] : -1; };
-    auto load = [&](const int8_t *cache, int j, int i, int page) {
-      if (page < 0 || page >= a.blocks || !in_head) return make_uint4(0, 0, 0, 0);
-      const int p = j * KT + brow + i * PER;
-      return __ldg(reinterpret_cast<const uint4 *>(
-          cache + (((int64_t)page * a.nkv + h) * a.block + p % a.block) * a.hs + piece * 16));
+    // table entries from held on are no row's to see (or NaN rows')
+    const int held = min(a.width, (r.length + a.block - 1) / a.block);
+    const int page_bytes = a.nkv * a.block * a.hs, head_bytes = h * a.block * a.hs + piece * 16;
+    const int step_blocks = KT / a.block, step_rest = KT % a.block;
+    // a row's place: its block in the table, its position in the block
+    struct Place {
+      int block, at;
+    };
+    auto place_of = [&](int p) { return Place{p / a.block, p % a.block}; };
+    auto forward = [&](Place &p) {
+      p.block += step_blocks, p.at += step_rest;
+      if (p.at >= a.block) p.at -= a.block, p.block++;
+    };
+    auto page_of = [&](const Place &p) { return p.block < held ? table[p.block] : -1; };
+    auto load = [&](const int8_t *cache, int page, int at) {
+      if ((uint32_t)page >= (uint32_t)a.blocks || !in_head) return make_uint4(0, 0, 0, 0);
+      return __ldg(reinterpret_cast<const uint4 *>(cache + (int64_t)page * page_bytes + head_bytes + at * a.hs));
     };
     auto widened = [&](uint8_t *tile, int i, const uint4 &v) {
       const int row = brow + i * PER;
@@ -302,27 +363,32 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       *reinterpret_cast<uint4 *>(dst + (((c0 + 1) ^ (row & 7)) << 4)) =
           make_uint4(widen<0x4140>(w[2]), widen<0x4342>(w[2]), widen<0x4140>(w[3]), widen<0x4342>(w[3]));
     };
-    int page[R], next[R];
+    Place far[R];  // of the step after next
+    int next[R], next_at[R];  // the next step's blocks and places in them
     uint4 k[R], v[R];
-    auto unit_of = [&](int j, int i) { return j * KU + (brow + i * PER) / UNIT; };
 #pragma unroll
     for (int i = 0; i < R; i++) {
-      page[i] = most_steps > 0 ? page_of(unit_of(0, i)) : -1;
-      next[i] = most_steps > 1 ? page_of(unit_of(1, i)) : -1;
+      far[i] = place_of(brow + i * PER);
+      const int page = most_steps > 0 ? page_of(far[i]) : -1;
+      k[i] = load(a.kc, page, far[i].at), v[i] = load(a.vc, page, far[i].at);
+      forward(far[i]);
+      next[i] = most_steps > 1 ? page_of(far[i]) : -1, next_at[i] = far[i].at;
+      forward(far[i]);
     }
-#pragma unroll
-    for (int i = 0; i < R; i++) k[i] = load(a.kc, 0, i, page[i]), v[i] = load(a.vc, 0, i, page[i]);
     // threads 0..3: a unit's scales, one step ahead, its block two
+    Place sfar = place_of((tid & 3) * UNIT);
     int spage = -1;
     float ks = 0.0f, vs = 0.0f;
     auto scales = [&](int p) {
-      const bool ok = p >= 0 && p < a.blocks;
+      const bool ok = (uint32_t)p < (uint32_t)a.blocks;
       ks = ok ? a.ks[(int64_t)p * a.nkv + h] : __uint_as_float(0x7fffffffu);
       vs = ok ? a.vs[(int64_t)p * a.nkv + h] : __uint_as_float(0x7fffffffu);
     };
     if (tid < KU && most_steps > 0) {
-      scales(page_of(tid));
-      spage = most_steps > 1 ? page_of(KU + tid) : -1;
+      scales(page_of(sfar));
+      forward(sfar);
+      spage = page_of(sfar);
+      forward(sfar);
     }
     for (int j = 0; j < most_steps; j++) {
       const int slot = j % STAGES;
@@ -331,13 +397,14 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
 #pragma unroll
       for (int i = 0; i < R; i++) {
         widened(s.k[slot][0], i, k[i]);
-        if (more) k[i] = load(a.kc, j + 1, i, next[i]);
+        if (more) k[i] = load(a.kc, next[i], next_at[i]);
       }
 #pragma unroll
       for (int i = 0; i < R; i++) {
         widened(s.v[slot][0], i, v[i]);
-        if (more) v[i] = load(a.vc, j + 1, i, next[i]);
-        next[i] = j + 2 < most_steps ? page_of(unit_of(j + 2, i)) : -1;
+        if (more) v[i] = load(a.vc, next[i], next_at[i]);
+        next[i] = page_of(far[i]), next_at[i] = far[i].at;
+        forward(far[i]);
       }
       if (tid < KU) {
         // a key scale of 0 (a block of zeros) as the least: 0 times a masked -inf is no number
@@ -345,125 +412,176 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
         s.sc[slot][tid] = make_float4(c, __log2f(w), __fdiv_rn(1.0f, w), 0.0f);
         if (more) {
           scales(spage);
-          spage = j + 2 < most_steps ? page_of((j + 2) * KU + tid) : -1;
+          spage = page_of(sfar);
+          forward(sfar);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&s.kv_full[slot]);
     }
-  } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 12) {
-      const uint32_t id_s = idesc_f16(QT, KT), id_o = idesc_f16(QT, HP) | B_MAJOR_N;
-      const int ksteps = a.hs / 16;
-      auto issue_s = [&](int t, int j) {
-        const int slot = j % STAGES;
-        for (int part = 0; part < PARTS; part++)
-          for (int kk = 0; kk < ksteps; kk++)
-            mma_f16(tS(t, j & 1), desc_sw128(s.q[t][part][kk >> 2] + 32 * (kk & 3)),
-                    desc_sw128(s.k[slot][kk >> 2] + 32 * (kk & 3)), id_s, part > 0 || kk > 0);
-        mma_commit(&s.s_full[t][j & 1]);
-      };
-      auto issue_pv = [&](int t, int j) {
-        const int slot = j % STAGES;
-#pragma unroll
-        for (int part = 0; part < PARTS; part++)
-#pragma unroll
-          for (int kk = 0; kk < KT / 16; kk++)
-            mma_ts(tO(t), tS(t, j & 1) + 32 * part + 8 * kk, desc_head_major(s.v[slot][0] + 2048 * kk, KT * 128), id_o,
-                   j > 0 || part > 0 || kk > 0);
-        mma_commit(&s.pv_done[t][j & 1]);
-      };
-      bool ok = __all_sync(0xffffffffu, mbar_wait(&s.q_full, 0, error, 103));
-      for (int j = 0; ok && j < 2 && j < most_steps; j++) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&s.kv_full[j], 0, error, 104));
-        if (!ok) break;
-        fence_after();
-        if (lane == 0)
-          for (int t = 0; t < 2; t++)
-            if (j < steps[t]) issue_s(t, j);
-        __syncwarp();
-      }
-      for (int j = 0; ok && j < most_steps; j++) {
-        const int ahead = (j + 2) % STAGES;
-        for (int t = 0; ok && t < 2; t++) {
-          if (j >= steps[t]) continue;
-          ok = __all_sync(0xffffffffu, mbar_wait(&s.p_full[t][j & 1], (j >> 1) & 1, error, 106));
+  } else if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    // A warp each for the scores' products and for the values', of each tile, and one thread of it: what such a thread waits
+    // for and works out between products takes a few hundred cycles, in which the others keep the tensor cores busy. What
+    // it computes for a product is a sum: the operands' descriptors are the first ones', with a multiple of 16 bytes added
+    // to the address in their low bits.
+    const int t = (warp - 16) >> 1;
+    if (t < TILES && elected()) {
+      constexpr int PART = S::CHUNKS * QT * 128 / 16, STAGE = S::CHUNKS * KT * 128 / 16;
+      bool ok = true;
+      auto wait = [&](uint64_t *bar, uint32_t parity, int code) { ok = ok && mbar_wait(bar, parity, error, code); };
+      if ((warp & 1) == 0) {
+        const uint32_t id_s = idesc_f16(QT, KT);
+        const uint64_t q0 = desc_sw128(s.q[t][0][0]), k0 = desc_sw128(s.k[0][0]);
+        wait(&s.q_full, 0, 103);
+        for (int j = 0; j < steps[t]; j++) {
+          wait(&s.kv_full[j % STAGES], (j / STAGES) & 1, 104);
+          wait(&s.pv_done[t][j % SBUF], ((j / SBUF) & 1) ^ 1, 107);  // the buffer's last weights have been used
           if (!ok) break;
           fence_after();
-          if (lane == 0) issue_pv(t, j);
-          __syncwarp();
-          if (j + 2 < steps[t]) {
-            // (the scores' buffer holds P until P V is done)
-            ok = mbar_wait(&s.pv_done[t][j & 1], (j >> 1) & 1, error, 107) &&
-                 mbar_wait(&s.kv_full[ahead], ((j + 2) / STAGES) & 1, error, 108);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            fence_after();
-            if (lane == 0) issue_s(t, j + 2);
-            __syncwarp();
-          }
+          const uint32_t d = tS(t, j % SBUF);
+          const uint64_t kd = k0 + (j % STAGES) * STAGE;
+          mma_ss<false>(d, q0, kd, id_s);
+#pragma unroll
+          for (int part = 0; part < PARTS; part++)
+#pragma unroll
+            for (int kk = 0; kk < HP / 16; kk++)
+              if (part > 0 || kk > 0)
+                mma_ss<true>(d, q0 + part * PART + (kk >> 2) * (QT * 8) + 2 * (kk & 3), kd + (kk >> 2) * (KT * 8) + 2 * (kk & 3),
+                             id_s);
+          mma_commit(&s.s_full[t][j % SBUF]);
         }
-        // every product that reads the stage is issued: it is free when they are done
-        if (ok && lane == 0) mma_commit(&s.kv_empty[j % STAGES]);
-        __syncwarp();
+      } else {
+        const uint32_t id_o = idesc_f16(QT, HP) | B_MAJOR_N;
+        const uint64_t v0 = desc_head_major(s.v[0][0], KT * 128);
+        for (int j = 0; j < most_steps; j++) {
+          if (j >= steps[t]) {
+            // the other tile's alone (an arrival a step, so not before the step is there)
+            wait(&s.kv_full[j % STAGES], (j / STAGES) & 1, 108);
+            if (!ok) break;
+            mbar_arrive(&s.kv_empty[j % STAGES]);
+            continue;
+          }
+          wait(&s.p_full[t][j % SBUF], (j / SBUF) & 1, 106);
+          if (!HALF) wait(&s.o_free[j & 1], ((j >> 1) & 1) ^ 1, 105);
+          if (!ok) break;
+          fence_after();
+          const uint32_t d = tO(HALF ? t : j & 1), p = tS(t, j % SBUF);
+          const uint64_t vd = v0 + (j % STAGES) * STAGE;
+          if (HALF && j > 0) mma_ts<true>(d, p, vd, id_o);
+          else mma_ts<false>(d, p, vd, id_o);
+#pragma unroll
+          for (int part = 0; part < PARTS; part++)
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; kk++)
+              if (part > 0 || kk > 0) mma_ts<true>(d, p + 32 * part + 8 * kk, vd + 128 * kk, id_o);
+          mma_commit(&s.pv_done[t][j % SBUF]);
+          mma_commit(&s.kv_empty[j % STAGES]);  // (this step's scores came before its weights)
+        }
       }
-      // every product issued has completed before the block frees TMEM
-      if (lane == 0) mma_commit(&s.mma_done);
+      mma_commit(&s.mma_done);
+    }
+    __syncwarp();
+    // every product issued has completed before the block frees TMEM
+    if (warp == 16) mbar_wait(&s.mma_done, 0, error, 114);
+  } else if (!HALF && warp >= 12) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    // ---- float32: the rows' sums, a step's product at a time
+    const int n = steps[0];
+    float acc[HP];
+#pragma unroll
+    for (int i = 0; i < HP; i++) acc[i] = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < n && ok; j++) {
+      ok = mbar_wait(&s.by_full[j & 3], (j >> 2) & 1, error, 121);
+      ok = mbar_wait(&s.pv_done[0][j % SBUF], (j / SBUF) & 1, error, 122) && ok;
+      ok = __all_sync(0xffffffffu, ok);
+      const float by = s.by[j & 3][y];
+      const uint64_t by2 = f2(by, by);
+      fence_after();
+#pragma unroll
+      for (int ch = 0; ch < HP / 16; ch++) {
+        uint32_t o[16];
+        tmem_ld<16>(tO(j & 1) + lane_base + ch * 16, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const uint64_t z = fma_2(f2(acc[ch * 16 + i], acc[ch * 16 + i + 1]), by2,
+                                   f2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])));
+          acc[ch * 16 + i] = lo_of(z), acc[ch * 16 + i + 1] = hi_of(z);
+        }
+      }
+      fence_before();
       __syncwarp();
-      mbar_wait(&s.mma_done, 0, error, 114);
+      if (lane == 0) mbar_arrive(&s.o_free[j & 1]);
+    }
+    ok = mbar_wait(&s.l_full, 0, error, 123) && ok;
+    const float by = inverse(s.l[y], ok);
+    if (on) {
+#pragma unroll
+      for (int d = 0; d < HP; d += 8)
+        if (d < a.hs) {
+          float z[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) z[e] = by == 0.0f ? 0.0f : acc[d + e] * by;
+          put(d, z);
+        }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
-    // ---- the softmax of tile t: thread y has row row0 + t * QT + y, TMEM lane y
-    const int t = (warp - 4) >> 2, y = tid - 128 * (t + 1), x = row0 + t * QT + y;
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const bool on = x < rows;
-    const int token = on ? x / a.group : 0, head = h * a.group + (on ? x % a.group : 0);
-    const int pos = on ? r.length - r.fresh + token : -1;
-    // its query, as float16 (float32: by a power of two into (0, 2), in two parts) in the swizzled layout
+    if (HALF && warp >= 12) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    // ---- the softmax of tile t_own. Its queries first, as float16 (float32: by a power of two into (0, 2), in two parts)
+    // in the swizzled layout
+    const int t = t_own;
     float qf = 1.0f;
     {
-      const int64_t off = (int64_t)(r.first + token) * a.q_stride + (int64_t)head * a.hs;
-      float f = 1.0f;
-      if (!HALF) {
-        const float4 *src = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + off);
-        float top = 0.0f;
-#pragma unroll 8
-        for (int d = 0; d < a.hs / 4; d++) {
-          const float4 z = on ? src[d] : make_float4(0, 0, 0, 0);
-          top = fmaxf(fmaxf(fmaxf(top, fabsf(z.x)), fmaxf(fabsf(z.y), fabsf(z.z))), fabsf(z.w));
-        }
-        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
-        f = __uint_as_float((uint32_t)(127 - e) << 23);
-        qf = __uint_as_float((uint32_t)(127 + e) << 23);
-      }
-#pragma unroll 4
-      for (int d = 0; d < a.hs; d += 8) {
+      // a row by LANES threads, 8 values each, all rows' loads in flight
+      constexpr int LANES = HP / 8, AT_ONCE = 128 / LANES;
+      const int col = y % LANES * 8, sub = y / LANES;
+#pragma unroll (HALF ? 16 : 4)
+      for (int row = sub; row < QT; row += AT_ONCE) {
+        const int x = row0 + t * QT + row;
+        const int64_t off = (int64_t)(r.first + (x < rows ? x / a.group : 0)) * a.q_stride +
+                            (int64_t)(h * a.group + (x < rows ? x % a.group : 0)) * a.hs + col;
+        const bool in = x < rows && col < a.hs;  // (zeros past the head, as the keys have there)
         uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (on) {
-          if (HALF) {
-            hi = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __half *>(a.q) + off + d);
-          } else {
-            const float4 *src = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + off + d);
-            const float4 z0 = src[0], z1 = src[1];
-            const float z[8] = {z0.x * f, z0.y * f, z0.z * f, z0.w * f, z1.x * f, z1.y * f, z1.z * f, z1.w * f};
-            uint32_t p[4], q[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              p[i] = pack(z[2 * i], z[2 * i + 1]);
-              const float2 b = unpack(p[i]);
-              q[i] = pack(z[2 * i] - b.x, z[2 * i + 1] - b.y);
-            }
-            hi = make_uint4(p[0], p[1], p[2], p[3]), lo = make_uint4(q[0], q[1], q[2], q[3]);
+        if (HALF) {
+          if (in) hi = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __half *>(a.q) + off);
+        } else {
+          float4 z0 = make_float4(0, 0, 0, 0), z1 = z0;
+          if (in) {
+            const float4 *src = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + off);
+            z0 = src[0], z1 = src[1];
           }
+          float z[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w}, top = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(z[i]));
+#pragma unroll
+          for (int d = LANES / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
+          const float f = __uint_as_float((uint32_t)(127 - e) << 23);
+          if (col == 0) s.l[row] = __uint_as_float((uint32_t)(127 + e) << 23);
+          uint32_t p[4], q[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            z[2 * i] *= f, z[2 * i + 1] *= f;
+            p[i] = pack(z[2 * i], z[2 * i + 1]);
+            const float2 b = unpack(p[i]);
+            q[i] = pack(z[2 * i] - b.x, z[2 * i + 1] - b.y);
+          }
+          hi = make_uint4(p[0], p[1], p[2], p[3]), lo = make_uint4(q[0], q[1], q[2], q[3]);
         }
-        const int at = y * 128 + ((((d & 63) >> 3) ^ (y & 7)) << 4);
-        *reinterpret_cast<uint4 *>(&s.q[t][0][d >> 6][at]) = hi;
-        if (!HALF) *reinterpret_cast<uint4 *>(&s.q[t][PARTS - 1][d >> 6][at]) = lo;
+        const int at = row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4);
+        *reinterpret_cast<uint4 *>(&s.q[t][0][col >> 6][at]) = hi;
+        if (!HALF) *reinterpret_cast<uint4 *>(&s.q[t][PARTS - 1][col >> 6][at]) = lo;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&s.q_full);
+      if (!HALF) {
+        // the rows' powers of two, among the four warps (l is for the sums later)
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        qf = s.l[y];
+      }
     }
     const int first_pos = r.length - r.fresh + (row0 + t * QT) / a.group;  // the tile's first row's
     const uint32_t o_col = tO(t) + lane_base;
@@ -471,59 +589,78 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     const int n = steps[t];
     bool ok = true;
     for (int j = 0; j < n && ok; j++) {
-      ok = mbar_wait(&s.s_full[t][j & 1], (j >> 1) & 1, error, 116);
-      // (kv_full of this step completed before its scores: the scales, written before it, are there)
+      ok = mbar_wait(&s.s_full[t][j % SBUF], (j / SBUF) & 1, error, 116);
+      // (complete before the scores were begun: its scales are there)
       ok = mbar_wait(&s.kv_full[j % STAGES], (j / STAGES) & 1, error, 117) && ok;
       ok = __all_sync(0xffffffffu, ok);
       fence_after();
-      const float4 *sc = s.sc[j % STAGES];
+      // where a row's maximum moves; by < 0: nowhere in the warp
+      auto settle = [&](float by) {
+        if (!HALF) {
+          s.by[j & 3][y] = by < 0.0f ? 1.0f : by;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.by_full[j & 3]);
+        } else if (by >= 0.0f && j > 0) {  // (whole warps come here: TMEM is read and written by whole warps)
+          // O holds the steps so far: it goes to the new maxima once the last P V is done
+          mbar_wait(&s.pv_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1, error, 109);
+          __syncwarp();
+          fence_after();
+#pragma unroll
+          for (int ch = 0; ch < HP / 32; ch++) {
+            float o[32];
+            ld32(o_col + ch * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] *= by;
+            st32(o_col + ch * 32, o);
+          }
+        }
+        return by;
+      };
       // (rows that don't exist have pos -1: nothing of a step is theirs, and nothing of theirs is written)
-      if (j * KT + KT - 1 > first_pos)
-        softmax_step<HP, HALF, true>(tS(t, j & 1) + lane_base, o_col, sc, qf, pos, j * KT, j, m, l, &s.pv_done[t], error);
-      else
-        softmax_step<HP, HALF, false>(tS(t, j & 1) + lane_base, o_col, sc, qf, pos, j * KT, j, m, l, &s.pv_done[t], error);
+      const uint32_t from = tS(t, j % SBUF) + lane_base;
+      const float4 *sc = s.sc[j % STAGES];
+      if (j * KT + KT - 1 > first_pos) softmax_step<HP, HALF, true>(from, sc, qf, pos - j * KT, m, l, settle);
+      else softmax_step<HP, HALF, false>(from, sc, qf, 0, m, l, settle);
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s.p_full[t][j & 1]);
+      if (lane == 0) mbar_arrive(&s.p_full[t][j % SBUF]);
     }
-    if (n > 0) {
-      ok = mbar_wait(&s.pv_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1, error, 118) && ok;
+    if (!HALF) {
+      s.l[y] = ok ? l : __uint_as_float(0x7fffffffu);
       __syncwarp();
-      fence_after();
-    }
-    float by = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-    if (!ok || pos >= cap) by = __uint_as_float(0x7fffffffu);  // a wait gave up; a position past the table's row
-    const int64_t off = (int64_t)(r.first + token) * a.out_stride + (int64_t)head * a.hs;
-#pragma unroll
-    for (int ch = 0; ch < HP / 32; ch++) {
-      float o[32];
-      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.l_full);
+    } else {
       if (n > 0) {
-        ld32(o_col + ch * 32, o);
-        tmem_wait_ld();
+        ok = mbar_wait(&s.pv_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1, error, 118) && ok;
+        __syncwarp();
+        fence_after();
       }
-      if (!on) continue;
+      const float by = inverse(l, ok);
 #pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        const int d = ch * 32 + i;
-        if (d >= a.hs) break;
-        float z[8];
+      for (int ch = 0; ch < HP / 32; ch++) {
+        float o[32];
+        __syncwarp();
+        if (n > 0) {
+          ld32(o_col + ch * 32, o);
+          tmem_wait_ld();
+        }
+        if (on) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) z[e] = n > 0 && by != 0.0f ? o[i + e] * by : by;
-        if (HALF) {
-          *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(a.out) + off + d) =
-              make_uint4(pack(z[0], z[1]), pack(z[2], z[3]), pack(z[4], z[5]), pack(z[6], z[7]));
-        } else {
-          float4 *dst = reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + off + d);
-          dst[0] = make_float4(z[0], z[1], z[2], z[3]);
-          dst[1] = make_float4(z[4], z[5], z[6], z[7]);
+          for (int i = 0; i < 32; i += 8)
+            if (ch * 32 + i < a.hs) {
+              float z[8];
+#pragma unroll
+              for (int e = 0; e < 8; e++) z[e] = n > 0 && by != 0.0f ? o[i + e] * by : by;
+              put(ch * 32 + i, z);
+            }
         }
       }
     }
   }
   fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
@@ -531,14 +668,15 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
 
 template <int HP, bool HALF>
 int launch_tc(const Args &a, cudaStream_t stream) {
+  using S = Tc<HP, HALF>;
   auto kernel = cache8_attention_tc_kernel<HP, HALF>;
-  const size_t smem = sizeof(typename Tc<HP, HALF>::Smem) + 1024;
+  const size_t smem = sizeof(typename S::Smem) + 1024;
   B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  // pairs of tiles: all rows', and one more for every request that has any (at least rows_most + 1 rows each)
+  // groups of tiles: all rows', and one more for every request that has any (at least rows_most + 1 rows each)
   const int64_t rows = (int64_t)a.n * a.group, requests = rows / (a.rows_most + 1);
-  const int64_t pairs = rows / (2 * QT) + (requests < a.n_seqs ? requests : a.n_seqs);
-  if (pairs < 1) return 0;
-  launch(kernel, dim3((unsigned)pairs, a.nkv), dim3(THREADS), smem, stream, a);
+  const int64_t groups = rows / (S::TILES * QT) + (requests < a.n_seqs ? requests : a.n_seqs);
+  if (groups < 1) return 0;
+  launch(kernel, dim3((unsigned)(groups * a.nkv)), dim3(THREADS), smem, stream, a);
   B200_LAUNCHED("cache8_attention_tc");
   return 0;
 }
