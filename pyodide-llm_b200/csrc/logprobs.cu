@@ -392,9 +392,11 @@ __global__ void __launch_bounds__(T, RESIDENT) logprobs_kernel(const Args a) {
           }
       }
       if (reaches && edge_id >= 0) list(edge, edge_id);
-      // the other groups of a thread with a third one: its warp reads them together
+      // the other groups of a thread with a third one: its warp reads them together (values equal to the bound only as long
+      // as their list has room: past it they are looked for in order)
       __syncwarp();
-      for (uint32_t more = __ballot_sync(0xffffffffu, reaches && third >= floor); more; more &= more - 1) {
+      auto wanted = [&](float y) { return y > floor || (y == floor && *(volatile int *)equals_s <= EQUAL); };
+      for (uint32_t more = __ballot_sync(0xffffffffu, reaches && wanted(third)); more; more &= more - 1) {
         const int whose = __ffs(more) - 1;
         const int first = __shfl_sync(0xffffffffu, best_group, whose), then = __shfl_sync(0xffffffffu, second_group, whose);
         const int v0 = r.v0 - lane + whose;
@@ -404,7 +406,7 @@ __global__ void __launch_bounds__(T, RESIDENT) logprobs_kernel(const Args a) {
           values_of(src[v0 + i * T], y);
 #pragma unroll
           for (int j = 0; j < VW; j++) most = fmaxf(most, y[j]);
-          if (most >= floor && i / GROUP != first && i / GROUP != then)
+          if (wanted(most) && i / GROUP != first && i / GROUP != then)
 #pragma unroll 1
             for (int j = 0; j < VW; j++) list((float)r.x[r.lead + (v0 + i * T) * VW + j], r.lead + (v0 + i * T) * VW + j);
         }
