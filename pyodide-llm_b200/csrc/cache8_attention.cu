@@ -100,15 +100,18 @@ __device__ __forceinline__ void block_scan(int64_t (&v)[2], int64_t (&all)[2], i
 template <int HSEG, int RT, bool HALF>
 struct Shape {
   static constexpr int HP = HSEG * 64;              // the head size, padded
-  static constexpr int NT = RT / 8;                 // row tiles of the instruction
+  // Four rows of float32: the instruction's eight columns hold the rows' high parts and their low parts, so one product
+  // does for both (mma.sync runs at a ninth of the tcgen05 rate here, 0.22 an SM and cycle: 32 a unit were 70 of 150 us)
+  static constexpr bool BOTH = RT == 4;
+  static constexpr int NT = BOTH ? 1 : RT / 8;      // row tiles of the instruction
   static constexpr int KSTEPS = HSEG * 4;           // instructions along the head
   static constexpr int VB = HSEG % 2 ? 8 : 16;      // bytes of a lane's piece of a value row
   static constexpr int VN = HP / (8 * VB);          // pieces
   static constexpr int STAGE = HSEG * 2048;         // bytes of a unit's keys and values
   static constexpr int STAGES = RING / STAGE;       // 8, 4, 2, 2
-  static constexpr int QREGS = KSTEPS * NT * (HALF ? 2 : 4);
+  static constexpr int QREGS = KSTEPS * NT * (HALF || BOTH ? 2 : 4);
   static constexpr bool QREG = QREGS <= 32;         // the query fragments in registers, else in shared memory
-  static constexpr int MINB = HSEG * RT <= 16 ? 3 : 2;
+  static constexpr int MINB = HSEG * (BOTH ? 8 : RT) <= 16 ? 3 : 2;
   struct Smem {
     alignas(16) uint8_t ring[WARPS][RING];          // later the warps' sums [WARPS][RT][HP]
     alignas(16) uint4 qf[QREG ? 1 : KSTEPS * NT * 32];
@@ -119,10 +122,13 @@ struct Shape {
   };
 };
 
-template <int HSEG, int RT, bool HALF>
+// WHOLE: the head size is HSEG * 64 (copies then need no condition and only immediate offsets)
+template <int HSEG, int RT, bool HALF, bool WHOLE>
 __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8_attention_kernel(const Args a) {
   using S = Shape<HSEG, RT, HALF>;
   constexpr int NT = S::NT, HP = S::HP, STAGES = S::STAGES;
+  constexpr bool BOTH = S::BOTH, PAIR = !HALF && !BOTH;  // PAIR: the low parts in instructions of their own
+  const int hs = WHOLE ? HP : a.hs;
   extern __shared__ __align__(16) uint8_t raw[];
   typename S::Smem &sm = *reinterpret_cast<typename S::Smem *>(raw);
   pdl_begin();
@@ -179,6 +185,8 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
     if (blockIdx.x == 0 && h == 0 && tid == 0) a.meta[-1] = make_int4((int)carry[1], 0, 0, 0);
   }
 
+  const int page_bytes = a.nkv * a.block * hs;
+  const int step_blocks = WARPS * UNIT / a.block, step_rest = WARPS * UNIT % a.block;  // a warp's way to its next unit
   const uint32_t ring = smem_addr(sm.ring[warp]);
   uint8_t *ring_p = sm.ring[warp];
   while (at < end) {
@@ -201,16 +209,19 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
     const int first = r.length - r.fresh + x0 / a.group;                       // the first row's
     const int u_end = min(u1, (min(last + 1, cap) + UNIT - 1) / UNIT);         // no row sees further units
 
+    // this lane's column p of row tile t, as a row of the tile
+    auto row_of = [&](int t, int p) { return BOTH ? 2 * (c & 1) + p : 8 * t + 2 * c + p; };
     // query fragments: lane (g, c) holds, for row g of row tile t, the head's values 64 j + 16 c + 4 w .. + 3
-    uint32_t qh[S::QREG ? S::KSTEPS * NT : 1][2], ql[S::QREG && !HALF ? S::KSTEPS * NT : 1][2];
+    // (BOTH: the high parts of row g, the low ones of row g - 4)
+    uint32_t qh[S::QREG ? S::KSTEPS * NT : 1][2], ql[S::QREG && PAIR ? S::KSTEPS * NT : 1][2];
     float qf[NT][2];  // what the scores of this lane's columns (rows 2 c, 2 c + 1 of row tile t) are to be scaled by
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const int x = x0 + 8 * t + g;
+      const int x = x0 + (BOTH ? g & 3 : 8 * t + g);
       const bool on = x < rows;
       const int64_t off = (int64_t)(r.first + (on ? x / a.group : 0)) * a.q_stride +
-                          (int64_t)(h * a.group + (on ? x % a.group : 0)) * a.hs;
+                          (int64_t)(h * a.group + (on ? x % a.group : 0)) * hs;
       float f = 1.0f, back = 1.0f;
       if (!HALF) {
         // each row by a power of two into (0, 2): float16 holds 22 bits of it in two parts
@@ -219,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
 #pragma unroll
         for (int j = 0; j < HSEG; j++) {
           const int d = 64 * j + 16 * c;
-          if (on && d < a.hs) {
+          if (on && d < hs) {
 #pragma unroll
             for (int w = 0; w < 4; w++) {
               const float4 v = *reinterpret_cast<const float4 *>(src + d + 4 * w);
@@ -233,12 +244,12 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
         f = __uint_as_float((uint32_t)(127 - e) << 23);
         back = __uint_as_float((uint32_t)(127 + e) << 23);
       }
-      qf[t][0] = __shfl_sync(0xffffffffu, back, 8 * c) * a.scale;
-      qf[t][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4) * a.scale;
+      qf[t][0] = __shfl_sync(0xffffffffu, back, BOTH ? 8 * (c & 1) : 8 * c) * a.scale;
+      qf[t][1] = __shfl_sync(0xffffffffu, back, BOTH ? 8 * (c & 1) + 4 : 8 * c + 4) * a.scale;
 #pragma unroll
       for (int j = 0; j < HSEG; j++) {
         const int d = 64 * j + 16 * c;
-        const bool in = on && d < a.hs;
+        const bool in = on && d < hs;
 #pragma unroll
         for (int w = 0; w < 4; w++) {
           uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
@@ -258,9 +269,10 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
             }
           }
           const int k = (4 * j + w) * NT + t;
+          if (BOTH && g >= 4) hi[0] = lo[0], hi[1] = lo[1];
           if (S::QREG) {
             qh[S::QREG ? k : 0][0] = hi[0], qh[S::QREG ? k : 0][1] = hi[1];
-            if (!HALF) ql[S::QREG && !HALF ? k : 0][0] = lo[0], ql[S::QREG && !HALF ? k : 0][1] = lo[1];
+            if (PAIR) ql[S::QREG && PAIR ? k : 0][0] = lo[0], ql[S::QREG && PAIR ? k : 0][1] = lo[1];
           } else if (warp == 0) {
             sm.qf[S::QREG ? 0 : k * 32 + lane] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
           }
@@ -272,71 +284,84 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
     for (int t = 0; t < NT; t++)
 #pragma unroll
       for (int p = 0; p < 2; p++) {
-        const int x = x0 + 8 * t + 2 * c + p;
+        const int x = x0 + row_of(t, p);
         pos[t][p] = x < rows ? r.length - r.fresh + x / a.group : -1;
       }
     if (!S::QREG) __syncthreads();
 
     // ---- the units of this warp: u0 + warp, + WARPS, ...
-    float M[NT][2], l[NT][2], o[NT][HSEG * 4][4];
+    float M[NT][2], from[NT][2], l[NT][2], o[NT][HSEG * 4][4];  // (from: M, or 0 while that is -inf)
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       M[t][0] = M[t][1] = -INFINITY;
-      l[t][0] = l[t][1] = 0.0f;
+      l[t][0] = l[t][1] = from[t][0] = from[t][1] = 0.0f;
 #pragma unroll
       for (int m = 0; m < HSEG * 4; m++) o[t][m][0] = o[t][m][1] = o[t][m][2] = o[t][m][3] = 0.0f;
     }
+    // The ring's front: the next unit to copy, its block's place in the table and its place in the block, and the id of
+    // that block (read one unit ahead).
     const int32_t *table = a.tables + (int64_t)req * a.width;
-    auto page_of = [&](int u) { return u < u_end ? table[u * UNIT / a.block] : -1; };
-    auto issue = [&](int u, int slot, int page) {
-      if (u < u_end) {
-        const bool ok = page >= 0 && page < a.blocks;
-        const int64_t ph = ok ? (int64_t)page * a.nkv + h : 0;
-        const int64_t row = ph * a.block + u * UNIT % a.block;
+    int front = u0 + warp, front_block = front * UNIT / a.block, front_at = front * UNIT % a.block;
+    auto forward = [&]() {
+      front += WARPS;
+      front_block += step_blocks, front_at += step_rest;
+      if (front_at >= a.block) front_at -= a.block, front_block++;
+    };
+    auto front_page = [&]() { return front < u_end ? table[front_block] : -1; };
+    int page = front_page();
+    const int8_t *k_lane = a.kc + (int64_t)h * a.block * hs + g * hs + 16 * c;
+    const int8_t *v_lane = a.vc + (int64_t)h * a.block * hs + 2 * c * hs + S::VB * g;
+    const float *s_lane = (lane == 1 ? a.vs : a.ks) + h;
+    auto issue = [&](int slot) {
+      const int mine = page, at = front_at;
+      const bool there = front < u_end, ok = (uint32_t)mine < (uint32_t)a.blocks;
+      forward();
+      page = front_page();
+      if (there) {
+        const int64_t off = ok ? (int64_t)mine * page_bytes + at * hs : 0;
+        const int8_t *k = k_lane + off, *v = v_lane + off;
         const uint32_t dst = ring + slot * S::STAGE + lane * 16;
 #pragma unroll
         for (int y = 0; y < 2; y++)
 #pragma unroll
           for (int j = 0; j < HSEG; j++) {
-            const int d = 64 * j + 16 * c;
-            const bool on = ok && d < a.hs;
-            copy<16>(dst + (y * HSEG + j) * 512, a.kc + (row + g + 8 * y) * a.hs + (on ? d : 0), on);
+            const bool on = ok && (WHOLE || 64 * j + 16 * c < hs);
+            copy<16>(dst + (y * HSEG + j) * 512, on || WHOLE ? k + y * 8 * hs + 64 * j : a.kc, on);
           }
         const uint32_t vdst = ring + slot * S::STAGE + HSEG * 1024 + lane * S::VB;
 #pragma unroll
         for (int y = 0; y < 4; y++)
 #pragma unroll
           for (int p = 0; p < S::VN; p++) {
-            const int d = p * 8 * S::VB + S::VB * g;
-            const bool on = ok && d < a.hs;
+            const bool on = ok && (WHOLE || p * 8 * S::VB + S::VB * g < hs);
             copy<S::VB>(vdst + (y * S::VN + p) * 32 * S::VB,
-                        a.vc + (row + 2 * c + (y & 1) + 8 * (y >> 1)) * a.hs + (on ? d : 0), on);
+                        on || WHOLE ? v + ((y & 1) + 8 * (y >> 1)) * hs + p * 8 * S::VB : a.vc, on);
           }
         // a table entry that is no block of the pool: NaN scales, so every row that sees it comes out NaN
         if (lane < 2) {
           float *dst_s = &sm.sc[warp][slot][lane];
-          if (ok) copy<4>(smem_addr(dst_s), (lane ? a.vs : a.ks) + ph, true);
+          if (ok) copy<4>(smem_addr(dst_s), s_lane + (int64_t)mine * a.nkv, true);
           else *dst_s = __uint_as_float(0x7fffffffu);
         }
       }
       copies_commit();
     };
     {
-      int u = u0 + warp;
-      int pages[STAGES];
 #pragma unroll
-      for (int s = 0; s < STAGES; s++) pages[s] = page_of(u + s * WARPS);
-#pragma unroll
-      for (int s = 0; s < STAGES - 1; s++) issue(u + s * WARPS, s, pages[s]);
-      int next = pages[STAGES - 1], slot = 0;
-      for (; u < u_end; u += WARPS) {
+      for (int s = 0; s < STAGES - 1; s++) issue(s);
+      int slot = 0;
+#pragma unroll 1
+      for (int u = u0 + warp; u < u_end; u += WARPS) {
         copies_wait<STAGES - 2>();
         __syncwarp();
         const float kscale = sm.sc[warp][slot][0], vscale = sm.sc[warp][slot][1];
-        // ---- scores: S^T = K Q^T, 16 positions x 8 rows an instruction tile
-        float s[NT][4];
+        // ---- scores: S^T = K Q^T, 16 positions x 8 rows an instruction tile (the two parts' sums apart: the
+        // instructions of one wait for one another)
+        float s[NT][4], s_lo[NT][4];
 #pragma unroll
-        for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[t][e] = s_lo[t][e] = 0.0f;
         const uint8_t *base = ring_p + slot * S::STAGE;
 #pragma unroll
         for (int j = 0; j < HSEG; j++) {
@@ -351,12 +376,13 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
             for (int t = 0; t < NT; t++) {
               const int k = (4 * j + w) * NT + t;
               if (S::QREG) {
-                mma(s[t], a0, a1, a2, a3, qh[S::QREG ? k : 0][0], qh[S::QREG ? k : 0][1]);
-                if (!HALF) mma(s[t], a0, a1, a2, a3, ql[S::QREG && !HALF ? k : 0][0], ql[S::QREG && !HALF ? k : 0][1]);
+                // (one part: even and odd steps' sums apart)
+                mma(!PAIR && (w & 1) ? s_lo[t] : s[t], a0, a1, a2, a3, qh[S::QREG ? k : 0][0], qh[S::QREG ? k : 0][1]);
+                if (PAIR) mma(s_lo[t], a0, a1, a2, a3, ql[S::QREG && PAIR ? k : 0][0], ql[S::QREG && PAIR ? k : 0][1]);
               } else {
                 const uint4 f = sm.qf[S::QREG ? 0 : k * 32 + lane];
-                mma(s[t], a0, a1, a2, a3, f.x, f.y);
-                if (!HALF) mma(s[t], a0, a1, a2, a3, f.z, f.w);
+                mma(!PAIR && (w & 1) ? s_lo[t] : s[t], a0, a1, a2, a3, f.x, f.y);
+                if (PAIR) mma(s_lo[t], a0, a1, a2, a3, f.z, f.w);
               }
             }
           }
@@ -364,28 +390,38 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
         // ---- weights. A value scale below 2^-100 counts as 2^-100 (a block of zeros has scale 0): what it weighs
         // is below any other block's last place
         const float vs = !(vscale < LEAST) ? vscale : LEAST;
-        const float lg = __log2f(vs), inv = __fdiv_rn(1.0f, vs);
-        const bool masked = u * UNIT + UNIT - 1 > first;
+        const float lg = __log2f(vs), inv = __frcp_rn(vs);
+        float f[NT][2], y[NT][4];  // (the exponents, as far as the maximum is concerned)
         bool up = false;
-        float f[NT][2];
-        bool on[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
 #pragma unroll
           for (int p = 0; p < 2; p++) f[t][p] = kscale * qf[t][p];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            on[t][e] = !masked || u * UNIT + g + 8 * (e >> 1) <= pos[t][e & 1];
-            up |= on[t][e] && __fmaf_rn(s[t][e], f[t][e & 1], lg) > M[t][e & 1] + RESCALE;
+            s[t][e] += s_lo[t][e];
+            if (BOTH) s[t][e] += __shfl_xor_sync(0xffffffffu, s[t][e], 2);  // the other part's sum
+            y[t][e] = __fmaf_rn(s[t][e], f[t][e & 1], lg);
           }
         }
+        const bool masked = u * UNIT + UNIT - 1 > first;
+        auto sees = [&](int t, int e) { return u * UNIT + g + 8 * (e >> 1) <= pos[t][e & 1]; };
+        if (masked) {
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[t][e] = sees(t, e) ? y[t][e] : -INFINITY;
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int p = 0; p < 2; p++) up |= fmaxf(y[t][p], y[t][2 + p]) > M[t][p] + RESCALE;
         if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
           for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int p = 0; p < 2; p++) {
-              float m = fmaxf(on[t][p] ? __fmaf_rn(s[t][p], f[t][p], lg) : -INFINITY,
-                              on[t][2 + p] ? __fmaf_rn(s[t][2 + p], f[t][p], lg) : -INFINITY);
+              float m = fmaxf(y[t][p], y[t][2 + p]);
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -395,26 +431,33 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
 #pragma unroll
               for (int x = 0; x < HSEG * 4; x++) o[t][x][p] *= by, o[t][x][2 + p] *= by;
               M[t][p] = m;
+              from[t][p] = m == -INFINITY ? 0.0f : m;
             }
         }
         uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-          float w[4];
+          float w[4], by[2] = {inv, inv};
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float m = M[t][e & 1] == -INFINITY ? 0.0f : M[t][e & 1];
-            w[e] = on[t][e] ? ex2(__fmaf_rn(s[t][e], f[t][e & 1], lg - m)) : 0.0f;
+          for (int e = 0; e < 4; e++) w[e] = ex2(__fmaf_rn(s[t][e], f[t][e & 1], lg - from[t][e & 1]));
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = sees(t, e) ? w[e] : 0.0f;
+            // (a row that sees nothing of the unit: 0 times a scale that may be NaN)
+#pragma unroll
+            for (int p = 0; p < 2; p++) by[p] = sees(t, p) ? inv : 0.0f;
           }
-          // (a row that sees nothing of the unit: 0 times a scale that may be NaN)
-          l[t][0] = __fmaf_rn(w[0] + w[2], on[t][0] || on[t][2] ? inv : 0.0f, l[t][0]);
-          l[t][1] = __fmaf_rn(w[1] + w[3], on[t][1] || on[t][3] ? inv : 0.0f, l[t][1]);
+          l[t][0] = __fmaf_rn(w[0] + w[2], by[0], l[t][0]);
+          l[t][1] = __fmaf_rn(w[1] + w[3], by[1], l[t][1]);
 #pragma unroll
-          for (int y = 0; y < 2; y++) {
-            const uint32_t hi = pack(w[2 * y], w[2 * y + 1]);
-            const float2 b = unpack(hi);
-            ph[t][y] = transposed(hi);
-            pl[t][y] = transposed(pack(w[2 * y] - b.x, w[2 * y + 1] - b.y));
+          for (int x = 0; x < 2; x++) {
+            uint32_t hi = pack(w[2 * x], w[2 * x + 1]), lo = 0;
+            if (!HALF) {
+              const float2 b = unpack(hi);
+              lo = pack(w[2 * x] - b.x, w[2 * x + 1] - b.y);
+            }
+            ph[t][x] = transposed(BOTH && c >= 2 ? lo : hi);
+            if (PAIR) pl[t][x] = transposed(lo);
           }
         }
         // ---- O^T += V^T P^T: lane (g, c)'s pieces of the rows of positions 2c, 2c + 1, 2c + 8, 2c + 9
@@ -434,24 +477,28 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
             }
           }
 #pragma unroll
-          for (int w = 0; w < S::VB / 4; w++)
+          for (int w = 0; w < S::VB / 4; w++) {
+            uint32_t a0[2], a1[2], a2[2], a3[2];
 #pragma unroll
             for (int y = 0; y < 2; y++) {
               const uint32_t p0 = (y ? interleave_hi(vw[0][w], vw[1][w]) : interleave_lo(vw[0][w], vw[1][w])) ^ 0x80808080u;
               const uint32_t p1 = (y ? interleave_hi(vw[2][w], vw[3][w]) : interleave_lo(vw[2][w], vw[3][w])) ^ 0x80808080u;
-              const uint32_t a0 = widen<0x4140>(p0), a1 = widen<0x4342>(p0), a2 = widen<0x4140>(p1), a3 = widen<0x4342>(p1);
-              const int m = p * S::VB / 2 + 2 * w + y;
+              a0[y] = widen<0x4140>(p0), a1[y] = widen<0x4342>(p0), a2[y] = widen<0x4140>(p1), a3[y] = widen<0x4342>(p1);
+            }
+            const int m = p * S::VB / 2 + 2 * w;
 #pragma unroll
-              for (int t = 0; t < NT; t++) {
-                mma(o[t][m], a0, a1, a2, a3, ph[t][0], ph[t][1]);
-                mma(o[t][m], a0, a1, a2, a3, pl[t][0], pl[t][1]);
+            for (int t = 0; t < NT; t++) {
+#pragma unroll
+              for (int y = 0; y < 2; y++) mma(o[t][m + y], a0[y], a1[y], a2[y], a3[y], ph[t][0], ph[t][1]);
+              if (PAIR) {
+#pragma unroll
+                for (int y = 0; y < 2; y++) mma(o[t][m + y], a0[y], a1[y], a2[y], a3[y], pl[t][0], pl[t][1]);
               }
             }
+          }
         }
         __syncwarp();  // every lane has read the slot's scales
-        const int ahead = u + (STAGES - 1) * WARPS;
-        issue(ahead, slot == 0 ? STAGES - 1 : slot - 1, next);
-        next = page_of(ahead + WARPS);
+        issue(slot == 0 ? STAGES - 1 : slot - 1);
         slot = slot + 1 == STAGES ? 0 : slot + 1;
       }
       copies_wait<0>();
@@ -465,15 +512,21 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
         l[t][p] += __shfl_xor_sync(0xffffffffu, l[t][p], 4);
         l[t][p] += __shfl_xor_sync(0xffffffffu, l[t][p], 8);
         l[t][p] += __shfl_xor_sync(0xffffffffu, l[t][p], 16);
-        if (g == 0) sm.ml[warp][8 * t + 2 * c + p][0] = M[t][p], sm.ml[warp][8 * t + 2 * c + p][1] = l[t][p];
+        if (g == 0) sm.ml[warp][row_of(t, p)][0] = M[t][p], sm.ml[warp][row_of(t, p)][1] = l[t][p];
       }
+    if (BOTH) {
+#pragma unroll
+      for (int m = 0; m < HSEG * 4; m++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[0][m][e] += __shfl_xor_sync(0xffffffffu, o[0][m][e], 2);
+    }
     __syncthreads();
     float *sums = reinterpret_cast<float *>(sm.ring);
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
       for (int p = 0; p < 2; p++) {
-        const int x = 8 * t + 2 * c + p;
+        const int x = row_of(t, p);
         float top = sm.ml[0][x][0];
 #pragma unroll
         for (int w = 1; w < WARPS; w++) top = fmaxf(top, sm.ml[w][x][0]);
@@ -484,12 +537,12 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
 #pragma unroll
           for (int w = 0; w < S::VB / 4; w++) {
             const int m = q * S::VB / 2 + 2 * w;
-            *reinterpret_cast<float4 *>(dst + q * 8 * S::VB + S::VB * g + 4 * w) = make_float4(
+            if (!BOTH || c < 2) *reinterpret_cast<float4 *>(dst + q * 8 * S::VB + S::VB * g + 4 * w) = make_float4(
                 o[t][m][p] * by, o[t][m][2 + p] * by, o[t][m + 1][p] * by, o[t][m + 1][2 + p] * by);
           }
       }
     __syncthreads();
-    const int quads = a.hs / 4;
+    const int quads = hs / 4;
     for (int i = tid; i < RT * quads; i += THREADS) {
       const int x = i / quads, d = (i - x * quads) * 4;
       if (x0 + x >= rows) break;
@@ -508,7 +561,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
       if (r.length - r.fresh + token >= cap) sum_l = __uint_as_float(0x7fffffffu);  // positions past the table's row
       if (spans == 1) {
         const float by = sum_l == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum_l);
-        const int64_t off = (int64_t)(r.first + token) * a.out_stride + (int64_t)head * a.hs + d;
+        const int64_t off = (int64_t)(r.first + token) * a.out_stride + (int64_t)head * hs + d;
         if (HALF) {
           *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(a.out) + off) =
               make_uint2(pack(sum.x * by, sum.y * by), pack(sum.z * by, sum.w * by));
@@ -518,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
         }
       } else {
         const int64_t row = ((blockIdx.x + tile_id) * a.nkv + h) * RT + x;
-        *reinterpret_cast<float4 *>(a.part + row * a.hs + d) = sum;
+        *reinterpret_cast<float4 *>(a.part + row * hs + d) = sum;
         if (d == 0) a.part_ml[row] = make_float2(top, sum_l);
       }
     }
@@ -531,73 +584,114 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
   }
 }
 
-// one row of a tile that several spans have worked on: its partial sums joined, in the spans' order within each warp
-// and the warps' at the end
+// The rows of tiles that several spans have worked on: the partial sums joined, a row by SHARE warps, each in the spans'
+// order, and those in theirs. SHARE 4 where there are few tiles (then it is the many spans of a long request that take
+// time), else 1.
 constexpr int CW = 4;  // warps
-template <int RT, bool HALF>
+template <int RT, int SHARE, bool HALF>
 __global__ void __launch_bounds__(CW * 32) cache8_combine_kernel(const Args a) {
   pdl_begin();
+  constexpr int ROWS = CW / SHARE;  // rows at a time
   __shared__ float acc[CW][256], ml[CW][2];
   const int tile_id = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int part = warp % SHARE;
   if (tile_id >= a.meta[-1].x) return;
   const int4 meta = a.meta[tile_id];
   if (meta.y < 2) return;
   const Request r = request_of(a, meta.z);
-  for (int x = blockIdx.z; x < RT; x += gridDim.z) {
-    const int row_of = meta.w * RT + x;
-    if (row_of >= r.fresh * a.group) break;
-    float M = -INFINITY, l = 0.0f, o[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) o[j] = 0.0f;
-    for (int s = warp; s < meta.y; s += CW) {
+  for (int x0 = blockIdx.z * ROWS; x0 < RT; x0 += gridDim.z * ROWS) {
+    const int x = x0 + warp / SHARE, row_of = meta.w * RT + x;
+    if (meta.w * RT + x0 >= r.fresh * a.group) break;
+    const bool on = row_of < r.fresh * a.group;
+    float M = -INFINITY, l = 0.0f;
+    float4 o[2];  // this lane's values 4 lane .. + 3, and 128 on
+    o[0] = o[1] = make_float4(0, 0, 0, 0);
+#pragma unroll 2
+    for (int s = part; s < meta.y && on; s += SHARE) {
       const int64_t row = (((int64_t)meta.x + s + tile_id) * a.nkv + h) * RT + x;
       const float2 v = a.part_ml[row];
+      float4 z[2];
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+        if (4 * lane + 128 * j < a.hs) z[j] = *reinterpret_cast<const float4 *>(a.part + row * a.hs + 4 * lane + 128 * j);
       const float m = fmaxf(M, v.x), by = M == m ? 1.0f : ex2(M - m), vy = v.x == m ? 1.0f : ex2(v.x - m);
       l = l * by + v.y * vy;
       M = m;
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (lane + 32 * j < a.hs) o[j] = o[j] * by + a.part[row * a.hs + lane + 32 * j] * vy;
+      for (int j = 0; j < 2; j++)
+        if (4 * lane + 128 * j < a.hs) {
+          o[j].x = o[j].x * by + z[j].x * vy, o[j].y = o[j].y * by + z[j].y * vy;
+          o[j].z = o[j].z * by + z[j].z * vy, o[j].w = o[j].w * by + z[j].w * vy;
+        }
     }
-    if (lane == 0) ml[warp][0] = M, ml[warp][1] = l;
+    if (SHARE > 1) {
+      if (lane == 0) ml[warp][0] = M, ml[warp][1] = l;
 #pragma unroll
-    for (int j = 0; j < 8; j++) acc[warp][lane + 32 * j] = o[j];
-    __syncthreads();
-    float top = ml[0][0], sum_l = 0.0f, by[CW];
+      for (int j = 0; j < 2; j++)
+        if (4 * lane + 128 * j < a.hs) *reinterpret_cast<float4 *>(&acc[warp][4 * lane + 128 * j]) = o[j];
+      __syncthreads();
+      float top = ml[warp - part][0];
 #pragma unroll
-    for (int w = 1; w < CW; w++) top = fmaxf(top, ml[w][0]);
+      for (int w = 1; w < SHARE; w++) top = fmaxf(top, ml[warp - part + w][0]);
+      l = 0.0f;
+      o[0] = o[1] = make_float4(0, 0, 0, 0);
+      if (part == 0) {
 #pragma unroll
-    for (int w = 0; w < CW; w++) {
-      by[w] = ml[w][0] == top ? 1.0f : ex2(ml[w][0] - top);
-      sum_l += ml[w][1] * by[w];
+        for (int w = 0; w < SHARE; w++) {
+          const float m = ml[warp + w][0], by = m == top ? 1.0f : ex2(m - top);
+          l += ml[warp + w][1] * by;
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+            if (4 * lane + 128 * j < a.hs) {
+              const float4 z = *reinterpret_cast<const float4 *>(&acc[warp + w][4 * lane + 128 * j]);
+              o[j].x += z.x * by, o[j].y += z.y * by, o[j].z += z.z * by, o[j].w += z.w * by;
+            }
+        }
+      }
     }
-    const float f = sum_l == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum_l);
-    const int token = row_of / a.group, head = h * a.group + row_of % a.group;
-    const int64_t off = (int64_t)(r.first + token) * a.out_stride + (int64_t)head * a.hs;
-    for (int d = threadIdx.x; d < a.hs; d += CW * 32) {
-      float sum = 0.0f;
+    if (part == 0 && on) {
+      const float f = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+      const int token = row_of / a.group, head = h * a.group + row_of % a.group;
+      const int64_t off = (int64_t)(r.first + token) * a.out_stride + (int64_t)head * a.hs + 4 * lane;
 #pragma unroll
-      for (int w = 0; w < CW; w++) sum += acc[w][d] * by[w];
-      if (HALF) reinterpret_cast<__half *>(a.out)[off + d] = __float2half_rn(sum * f);
-      else reinterpret_cast<float *>(a.out)[off + d] = sum * f;
+      for (int j = 0; j < 2; j++)
+        if (4 * lane + 128 * j < a.hs) {
+          if (HALF)
+            *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(a.out) + off + 128 * j) =
+                make_uint2(pack(o[j].x * f, o[j].y * f), pack(o[j].z * f, o[j].w * f));
+          else
+            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + off + 128 * j) =
+                make_float4(o[j].x * f, o[j].y * f, o[j].z * f, o[j].w * f);
+        }
     }
-    __syncthreads();  // acc and ml have been read
+    if (SHARE > 1) __syncthreads();  // acc and ml have been read
   }
 }
+template <int RT, bool HALF>
+int launch_combine(const Args &a, int64_t tiles, cudaStream_t stream) {
+  const bool few = tiles * a.nkv <= 64;
+  const dim3 grid((unsigned)tiles, a.nkv, few ? RT : 1);
+  launch(few ? cache8_combine_kernel<RT, CW, HALF> : cache8_combine_kernel<RT, 1, HALF>, grid, dim3(CW * 32), 0, stream, a);
+  B200_LAUNCHED("cache8_combine");
+  return 0;
+}
 
-// rows of a tile: 8 where the requests have that few on average, else 16 (a row tile costs instructions whether its
-// rows are there or not; a request with more rows takes several tiles)
-int rows_of_tile(int n, int n_seqs, int group) { return (int64_t)n * group <= 8 * (int64_t)n_seqs ? 8 : 16; }
+// rows of a tile: 8 where the requests have that few on average (float32: 4, see Shape), else 16 (a row tile costs
+// instructions whether its rows are there or not; a request with more rows takes several tiles)
+int rows_of_tile(int n, int n_seqs, int group, bool half) {
+  const int64_t rows = (int64_t)n * group;
+  return !half && rows <= 4 * (int64_t)n_seqs ? 4 : rows <= 8 * (int64_t)n_seqs ? 8 : 16;
+}
 
 struct Layout {
   int rt;
   int64_t tiles, parts;
   uint64_t ml_at, part_at, bytes;
 };
-Layout layout_of(int n, int n_seqs, int nh, int nkv, int hs) {
+Layout layout_of(int n, int n_seqs, int nh, int nkv, int hs, bool half) {
   Layout s;
   const int group = nh / nkv;
-  s.rt = rows_of_tile(n, n_seqs, group);
+  s.rt = rows_of_tile(n, n_seqs, group, half);
   s.tiles = ((int64_t)n * group + s.rt - 1) / s.rt + (n < n_seqs ? n : n_seqs);
   s.parts = s.tiles + (MOST_BLOCKS + nkv - 1) / nkv;
   const auto up = [](uint64_t x) { return (x + 255) / 256 * 256; };
@@ -607,16 +701,27 @@ Layout layout_of(int n, int n_seqs, int nh, int nkv, int hs) {
   return s;
 }
 
-template <int HSEG, int RT, bool HALF>
+template <int HSEG, int RT, bool HALF, bool WHOLE>
 int launch_attention8(const Args &a, int blocks_x, cudaStream_t stream) {
   using S = Shape<HSEG, RT, HALF>;
-  auto kernel = cache8_attention_kernel<HSEG, RT, HALF>;
+  auto kernel = cache8_attention_kernel<HSEG, RT, HALF, WHOLE>;
   B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename S::Smem)));
   const int most = 148 * S::MINB / a.nkv;
   launch(kernel, dim3(most < 1 ? 1 : most < blocks_x ? most : blocks_x, a.nkv), dim3(THREADS), sizeof(typename S::Smem),
          stream, a);
   B200_LAUNCHED("cache8_attention");
   return 0;
+}
+using Launch = int (*)(const Args &, int, cudaStream_t);
+template <int HSEG, int RT>
+Launch launch_of(bool half, bool whole) {
+  if (half) return whole ? launch_attention8<HSEG, RT, true, true> : launch_attention8<HSEG, RT, true, false>;
+  return whole ? launch_attention8<HSEG, RT, false, true> : launch_attention8<HSEG, RT, false, false>;
+}
+template <int HSEG>
+Launch launch_of(int rt, bool half, bool whole) {
+  if (rt == 4) return whole ? launch_attention8<HSEG, 4, false, true> : launch_attention8<HSEG, 4, false, false>;
+  return rt == 8 ? launch_of<HSEG, 8>(half, whole) : launch_of<HSEG, 16>(half, whole);
 }
 
 int check_sizes(const char *what, int n, int n_seqs, int nh, int nkv, int hs) {
@@ -639,11 +744,10 @@ using namespace b200;
 extern "C" int b200k_cache8_attention_scratch(int32_t n, int32_t n_seqs, int32_t nh, int32_t nkv, int32_t hs,
                                               int32_t half, uint64_t *bytes) {
   try {
-    (void)half;
     if (!bytes) return fail(B200FWD_EINVAL, "cache8_attention_scratch: null pointer");
     const int rc = check_sizes("cache8_attention_scratch", n, n_seqs, nh, nkv, hs);
     if (rc) return rc;
-    *bytes = layout_of(n, n_seqs, nh, nkv, hs).bytes;
+    *bytes = layout_of(n, n_seqs, nh, nkv, hs, half).bytes;
     return 0;
   } catch (...) {
     return fail(B200FWD_EINVAL, "cache8_attention_scratch: exception");
@@ -672,7 +776,7 @@ extern "C" int b200k_cache8_attention(void *out, const void *q, const int8_t *kc
       return fail(B200FWD_EINVAL, "cache8_attention: rows of q and out of nh * hs values at least, on 16 bytes");
     if (reinterpret_cast<uintptr_t>(scratch) % 256)
       return fail(B200FWD_EINVAL, "cache8_attention: scratch must be 256-byte aligned");
-    const Layout s = layout_of(n, n_seqs, nh, nkv, hs);
+    const Layout s = layout_of(n, n_seqs, nh, nkv, hs, half);
     uint8_t *base = reinterpret_cast<uint8_t *>(scratch);
     // blocks of tokens go to the tensor cores; where there is no more than a token a request on average, any request is
     // taken here, and one kernel less launched
@@ -684,23 +788,17 @@ extern "C" int b200k_cache8_attention(void *out, const void *q, const int8_t *kc
               1.4426950408889634f / sqrtf((float)hs)};
     const cudaStream_t st = as_stream(stream);
     const int hseg = (hs + 63) / 64, blocks_x = (MOST_BLOCKS + nkv - 1) / nkv;
-    using Launch = int (*)(const Args &, int, cudaStream_t);
-    static const Launch table[4][2][2] = {
-        {{launch_attention8<1, 8, false>, launch_attention8<1, 8, true>}, {launch_attention8<1, 16, false>, launch_attention8<1, 16, true>}},
-        {{launch_attention8<2, 8, false>, launch_attention8<2, 8, true>}, {launch_attention8<2, 16, false>, launch_attention8<2, 16, true>}},
-        {{launch_attention8<3, 8, false>, launch_attention8<3, 8, true>}, {launch_attention8<3, 16, false>, launch_attention8<3, 16, true>}},
-        {{launch_attention8<4, 8, false>, launch_attention8<4, 8, true>}, {launch_attention8<4, 16, false>, launch_attention8<4, 16, true>}}};
-    rc = table[hseg - 1][s.rt == 16][half ? 1 : 0](a, blocks_x, st);
+    const bool whole = hs % 64 == 0;
+    const Launch launch_units = hseg == 1   ? launch_of<1>(s.rt, half, whole)
+                                : hseg == 2 ? launch_of<2>(s.rt, half, whole)
+                                : hseg == 3 ? launch_of<3>(s.rt, half, whole)
+                                            : launch_of<4>(s.rt, half, whole);
+    rc = launch_units(a, blocks_x, st);
     if (!rc && prompts) rc = launch_attention8_prompts(a, half, st);
     if (rc) return rc;
-    // a row a thread block where there are few rows (the joining of a long request's many spans is what takes time
-    // then), else a tile
-    const dim3 grid((unsigned)s.tiles, nkv, s.tiles * nkv <= 1024 ? s.rt : 1);
-    auto combine = s.rt == 8 ? (half ? cache8_combine_kernel<8, true> : cache8_combine_kernel<8, false>)
-                             : (half ? cache8_combine_kernel<16, true> : cache8_combine_kernel<16, false>);
-    launch(combine, grid, dim3(CW * 32), 0, st, a);
-    B200_LAUNCHED("cache8_combine");
-    return 0;
+    return s.rt == 4   ? launch_combine<4, false>(a, s.tiles, st)
+           : s.rt == 8 ? (half ? launch_combine<8, true>(a, s.tiles, st) : launch_combine<8, false>(a, s.tiles, st))
+                       : (half ? launch_combine<16, true>(a, s.tiles, st) : launch_combine<16, false>(a, s.tiles, st));
   } catch (...) {
     return fail(B200FWD_EINVAL, "cache8_attention: exception");
   }
