@@ -2,13 +2,15 @@
 // many requests at once: out = sum_j p_j v_j, p = softmax_j(q . k_j / sqrt(hs)) over the positions j up to the row's
 // own, k_j = kscale[block][head] * int8, v_j likewise.
 //
-// A tile is RT (8 or 16) query rows of one request and kv head: its tokens' query heads that share the kv head, so
-// every byte of the cache is read once for all of them. The products run on mma.sync m16n8k16 (float16 operands,
-// float32 sums) with the cache as the 16-row operand: int8 integers are exact in float16, and the scales stay outside
-// (a block's key scale on its scores, its value scale within its weights), so the cache's values are never rounded.
-// Single tokens are bound by the cache's bytes; the tensor instructions' rate is no limit there.
-//  - float32 queries: q and the weights each as a float16 pair high + low (22 bits), two instructions for one;
-//    float16 queries are exact, and their weights are rounded to the same pairs: the outputs' own rounding remains.
+// A tile is RT (4, 8 or 16) query rows of one request and kv head: its tokens' query heads that share the kv head, so
+// every byte of the cache is read once for all of them. Both products run on mma.sync with the cache as the 16-row
+// operand; the scales stay outside (a block's key scale on its scores, its value scale within its weights), so the
+// cache's values are never rounded.
+//  - scores: the keys' bytes as they are (m16n8k32, signed bytes, exact int32 sums) with the queries in fixed point, each
+//    row by a power of two into (0, 2) and then as three digits of a byte, 21 bits behind the point: a column for each
+//    digit of each row, whose sums are put together in float32.
+//  - values: as float16 integers (exact), with the weights as a float16 pair high + low (float16 queries: one float16, half
+//    a step of the output's type).
 //  - weights: w = 2^(s + log2(vscale) - M), M a running maximum (per row) that moves only when it is passed by more
 //    than 2^8, and the row sum l += w / vscale: the block's value scale costs no operation per value, and what is
 //    rounded to float16 is relative to the largest term of the sum, whatever the scales.
@@ -16,8 +18,9 @@
 // spans, one for each thread block of a grid that fills the GPU once, so ragged requests balance and one long request
 // takes every SM. A tile cut by a span's end leaves partial sums (unnormalized, with M and l) that combine_kernel
 // joins in the order of the spans: results don't depend on timing.
-// Loads: each lane copies the bytes that it will multiply itself (cp.async into a ring of its own, so no thread waits
-// for another), stages deep enough to cover HBM's latency.
+// Loads: a warp copies a unit's rows by 16-byte pieces side by side (cp.async) into a ring of its own, so no warp waits for
+// another. (Each lane copying what it will multiply itself, 64-byte runs of eight rows, read 4.5 TB/s, this 5.8.) The
+// pieces of a row are swapped about by its number, so that neither the keys' reads nor the values' collide in a bank.
 #include <string>
 
 #include "cache8.h"
@@ -28,8 +31,21 @@ using namespace cache8;
 namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int RING = 16384;       // bytes of a warp's ring
 constexpr int MOST_BLOCKS = 148 * 3;  // thread blocks of a grid (resident at once)
+
+// Where a row's 16-byte piece q sits in the ring: 128-byte lines (of two rows of 64) with the pieces swapped by the row.
+// The keys' reads take pieces 4 j + c of rows place(g), g = 2 i and 2 i + 1 at a time, the values' 16 (8) bytes g of rows
+// place(2 c) or place(2 c + 1): each time in 128 bytes of different banks.
+template <int HSEG>
+__device__ __forceinline__ int piece_at(int row, int q) {
+  if (HSEG == 1) return (row >> 1) * 128 + (((((row & 1) << 2) + q) ^ (row & 6)) << 4);
+  return row * (HSEG == 2 ? 128 : 256) + (q >> 3) * 128 + (((q & 7) ^ (row & 7)) << 4);
+}
+// the position (of 8) that row g of a score tile stands for
+template <int HSEG>
+__device__ __forceinline__ int place(int g) {
+  return HSEG == 1 ? g : g & 1 ? (g + 4) & 7 : g;
+}
 
 template <int RT>
 __device__ __forceinline__ int tiles_of(const Args &a, const Request &r) {
@@ -41,14 +57,11 @@ __device__ __forceinline__ int units_of(const Args &a, const Request &r) {
   return max(1, (min(r.length, a.width * a.block) + UNIT - 1) / UNIT);
 }
 
-// BYTES (4, 8 or 16) to shared memory, zeros where !on (then nothing is read)
+// BYTES (4 or 16) to shared memory
 template <int BYTES>
-__device__ __forceinline__ void copy(uint32_t dst, const void *src, bool on) {
-  if (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(on ? BYTES : 0)
-                 : "memory");
+__device__ __forceinline__ void copy(uint32_t dst, const void *src) {
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -63,6 +76,25 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// D += A B of signed bytes, exact
+__device__ __forceinline__ void mma_i8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// four values of a query row
+template <bool HALF>
+__device__ __forceinline__ void query(const void *q, int64_t at, float (&z)[4]) {
+  if (HALF) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(reinterpret_cast<const __half *>(q) + at);
+    const float2 lo = unpack(v.x), hi = unpack(v.y);
+    z[0] = lo.x, z[1] = lo.y, z[2] = hi.x, z[3] = hi.y;
+  } else {
+    const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(q) + at);
+    z[0] = v.x, z[1] = v.y, z[2] = v.z, z[3] = v.w;
+  }
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
@@ -100,21 +132,24 @@ __device__ __forceinline__ void block_scan(int64_t (&v)[2], int64_t (&all)[2], i
 template <int HSEG, int RT, bool HALF>
 struct Shape {
   static constexpr int HP = HSEG * 64;              // the head size, padded
-  // Four rows of float32: the instruction's eight columns hold the rows' high parts and their low parts, so one product
-  // does for both (mma.sync runs at a ninth of the tcgen05 rate here, 0.22 an SM and cycle: 32 a unit were 70 of 150 us)
+  // Four rows of float32: the value products' eight columns hold the rows' weights' high parts and their low parts, so
+  // one instruction does for both.
   static constexpr bool BOTH = RT == 4;
-  static constexpr int NT = BOTH ? 1 : RT / 8;      // row tiles of the instruction
-  static constexpr int KSTEPS = HSEG * 4;           // instructions along the head
+  static constexpr int NT = BOTH ? 1 : RT / 8;      // row tiles of the value products
+  // the score products: 32 values of the head an instruction, columns by digit, then row
+  static constexpr int KSTEPS = HSEG * 2, CT = (3 * RT + 7) / 8;
   static constexpr int VB = HSEG % 2 ? 8 : 16;      // bytes of a lane's piece of a value row
   static constexpr int VN = HP / (8 * VB);          // pieces
-  static constexpr int STAGE = HSEG * 2048;         // bytes of a unit's keys and values
-  static constexpr int STAGES = RING / STAGE;       // 8, 4, 2, 2
-  static constexpr int QREGS = KSTEPS * NT * (HALF || BOTH ? 2 : 4);
+  static constexpr int ROW = HSEG <= 2 ? HP : 256;  // bytes of a row in the ring
+  static constexpr int STAGE = 2 * UNIT * ROW;      // of a unit's keys and values
+  static constexpr int RING = HSEG <= 2 ? 16384 : 24576;  // bytes of a warp's ring
+  static constexpr int STAGES = RING / STAGE;       // 8, 4, 3, 3
+  static constexpr int QREGS = KSTEPS * CT * 2;
   static constexpr bool QREG = QREGS <= 32;         // the query fragments in registers, else in shared memory
   static constexpr int MINB = HSEG * (BOTH ? 8 : RT) <= 16 ? 3 : 2;
   struct Smem {
     alignas(16) uint8_t ring[WARPS][RING];          // later the warps' sums [WARPS][RT][HP]
-    alignas(16) uint4 qf[QREG ? 1 : KSTEPS * NT * 32];
+    alignas(16) uint2 qf[QREG ? 1 : KSTEPS * CT * 32];
     float sc[WARPS][STAGES][2];                     // the units' scales
     float ml[WARPS][RT][2];
     int64_t part[2][WARPS];
@@ -211,71 +246,66 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
 
     // this lane's column p of row tile t, as a row of the tile
     auto row_of = [&](int t, int p) { return BOTH ? 2 * (c & 1) + p : 8 * t + 2 * c + p; };
-    // query fragments: lane (g, c) holds, for row g of row tile t, the head's values 64 j + 16 c + 4 w .. + 3
-    // (BOTH: the high parts of row g, the low ones of row g - 4)
-    uint32_t qh[S::QREG ? S::KSTEPS * NT : 1][2], ql[S::QREG && PAIR ? S::KSTEPS * NT : 1][2];
+    // Query fragments: lane (g, c) holds column 8 t + g of column tile t, digit (8 t + g) / RT of row (8 t + g) % RT, of the
+    // head's values 64 j + 16 c .. + 15, the bytes of keys that it copies.
+    uint32_t qd[S::QREG ? S::KSTEPS * S::CT : 1][2];
     float qf[NT][2];  // what the scores of this lane's columns (rows 2 c, 2 c + 1 of row tile t) are to be scaled by
     __syncthreads();
+    {
+      float f[NT], back[NT];
+      int64_t off[NT];
+      bool is[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-      const int x = x0 + (BOTH ? g & 3 : 8 * t + g);
-      const bool on = x < rows;
-      const int64_t off = (int64_t)(r.first + (on ? x / a.group : 0)) * a.q_stride +
-                          (int64_t)(h * a.group + (on ? x % a.group : 0)) * hs;
-      float f = 1.0f, back = 1.0f;
-      if (!HALF) {
-        // each row by a power of two into (0, 2): float16 holds 22 bits of it in two parts
-        const float *src = reinterpret_cast<const float *>(a.q) + off;
-        float top = 0.0f;
+      for (int t = 0; t < NT; t++) {
+        const int x = x0 + (BOTH ? g & 3 : 8 * t + g);
+        is[t] = x < rows;
+        off[t] = (int64_t)(r.first + (is[t] ? x / a.group : 0)) * a.q_stride + (int64_t)(h * a.group + (is[t] ? x % a.group : 0)) * hs;
+        // each row by a power of two into (0, 2)
+        uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < HSEG; j++) {
-          const int d = 64 * j + 16 * c;
-          if (on && d < hs) {
+        for (int j = 0; j < HSEG; j++)
+          if (is[t] && (WHOLE || 64 * j + 16 * c < hs)) {
 #pragma unroll
             for (int w = 0; w < 4; w++) {
-              const float4 v = *reinterpret_cast<const float4 *>(src + d + 4 * w);
-              top = fmaxf(fmaxf(fmaxf(top, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+              float z[4];
+              query<HALF>(a.q, off[t] + 64 * j + 16 * c + 4 * w, z);
+#pragma unroll
+              for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(z[i]) & 0x7fffffffu);
             }
           }
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
-        f = __uint_as_float((uint32_t)(127 - e) << 23);
-        back = __uint_as_float((uint32_t)(127 + e) << 23);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max((int)(top >> 23) - 127, -126), 126);
+        f[t] = __uint_as_float((uint32_t)(127 - e) << 23);
+        back[t] = __uint_as_float((uint32_t)(127 + e) << 23) * 4.76837158203125e-7f;  // 2^-21
+        if (top >= 0x7f800000u) back[t] = __uint_as_float(0x7fffffffu);  // (a row with an infinity or a NaN: NaN)
+        qf[t][0] = __shfl_sync(0xffffffffu, back[t], BOTH ? 8 * (c & 1) : 8 * c) * a.scale;
+        qf[t][1] = __shfl_sync(0xffffffffu, back[t], BOTH ? 8 * (c & 1) + 4 : 8 * c + 4) * a.scale;
       }
-      qf[t][0] = __shfl_sync(0xffffffffu, back, BOTH ? 8 * (c & 1) : 8 * c) * a.scale;
-      qf[t][1] = __shfl_sync(0xffffffffu, back, BOTH ? 8 * (c & 1) + 4 : 8 * c + 4) * a.scale;
 #pragma unroll
-      for (int j = 0; j < HSEG; j++) {
-        const int d = 64 * j + 16 * c;
-        const bool in = on && d < hs;
+      for (int t = 0; t < S::CT; t++) {
+        const int row_tile = BOTH ? 0 : t % NT, digit = BOTH ? 2 * t + (g >> 2) : t / NT;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-          uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
-          if (in) {
-            if (HALF) {
-              const uint2 v = *reinterpret_cast<const uint2 *>(reinterpret_cast<const __half *>(a.q) + off + d + 4 * w);
-              hi[0] = v.x, hi[1] = v.y;
-            } else {
-              const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + off + d + 4 * w);
-              const float y[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+        for (int i = 0; i < S::KSTEPS; i++) {
+          uint32_t word[2] = {0, 0};
+          const int d = 64 * (i / 2) + 16 * c + 8 * (i & 1);
+          if (is[row_tile] && digit < 3 && (WHOLE || d < hs)) {
 #pragma unroll
-              for (int p = 0; p < 2; p++) {
-                hi[p] = pack(y[2 * p], y[2 * p + 1]);
-                const float2 back2 = unpack(hi[p]);
-                lo[p] = pack(y[2 * p] - back2.x, y[2 * p + 1] - back2.y);
+            for (int y = 0; y < 2; y++) {
+              float z[4];
+              query<HALF>(a.q, off[row_tile] + d + 4 * y, z);
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                // q 2^21 = 65536 d0 + 256 d1 + d2, the digits from -128 to 127
+                const int whole = __float2int_rn(z[e] * f[row_tile] * 2097152.0f);
+                const int d2 = (int8_t)whole, upper = (whole - d2) >> 8, d1 = (int8_t)upper, d0 = (upper - d1) >> 8;
+                word[y] |= (uint32_t)((digit == 0 ? d0 : digit == 1 ? d1 : d2) & 255) << (8 * e);
               }
             }
           }
-          const int k = (4 * j + w) * NT + t;
-          if (BOTH && g >= 4) hi[0] = lo[0], hi[1] = lo[1];
-          if (S::QREG) {
-            qh[S::QREG ? k : 0][0] = hi[0], qh[S::QREG ? k : 0][1] = hi[1];
-            if (PAIR) ql[S::QREG && PAIR ? k : 0][0] = lo[0], ql[S::QREG && PAIR ? k : 0][1] = lo[1];
-          } else if (warp == 0) {
-            sm.qf[S::QREG ? 0 : k * 32 + lane] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
-          }
+          const int k = i * S::CT + t;
+          if (S::QREG) qd[S::QREG ? k : 0][0] = word[0], qd[S::QREG ? k : 0][1] = word[1];
+          else if (warp == 0) sm.qf[S::QREG ? 0 : k * 32 + lane] = make_uint2(word[0], word[1]);
         }
       }
     }
@@ -298,6 +328,16 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
 #pragma unroll
       for (int m = 0; m < HSEG * 4; m++) o[t][m][0] = o[t][m][1] = o[t][m][2] = o[t][m][3] = 0.0f;
     }
+    // this lane's places in the ring: of the pieces it copies, and of those it multiplies (of the first half of the rows)
+    int piece_to[HSEG * 2];
+#pragma unroll
+    for (int i = 0; i < HSEG * 2; i++) {
+      const int piece = i * 32 + lane, per = WHOLE ? HSEG * 4 : hs / 16;
+      piece_to[i] = piece_at<HSEG>(piece / per, piece % per);
+    }
+    const int k_from = piece_at<HSEG>(place<HSEG>(g), c);
+    const int v_from[2] = {piece_at<HSEG>(place<HSEG>(2 * c), S::VB == 16 ? g : g >> 1) + (S::VB == 16 ? 0 : (g & 1) * 8),
+                           piece_at<HSEG>(place<HSEG>(2 * c + 1), S::VB == 16 ? g : g >> 1) + (S::VB == 16 ? 0 : (g & 1) * 8)};
     // The ring's front: the next unit to copy, its block's place in the table and its place in the block, and the id of
     // that block (read one unit ahead).
     const int32_t *table = a.tables + (int64_t)req * a.width;
@@ -309,8 +349,8 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
     };
     auto front_page = [&]() { return front < u_end ? table[front_block] : -1; };
     int page = front_page();
-    const int8_t *k_lane = a.kc + (int64_t)h * a.block * hs + g * hs + 16 * c;
-    const int8_t *v_lane = a.vc + (int64_t)h * a.block * hs + 2 * c * hs + S::VB * g;
+    const int8_t *k_lane = a.kc + (int64_t)h * a.block * hs + lane * 16;
+    const int8_t *v_lane = a.vc + (int64_t)h * a.block * hs + lane * 16;
     const float *s_lane = (lane == 1 ? a.vs : a.ks) + h;
     auto issue = [&](int slot) {
       const int mine = page, at = front_at;
@@ -318,75 +358,82 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
       forward();
       page = front_page();
       if (there) {
-        const int64_t off = ok ? (int64_t)mine * page_bytes + at * hs : 0;
-        const int8_t *k = k_lane + off, *v = v_lane + off;
-        const uint32_t dst = ring + slot * S::STAGE + lane * 16;
+        if (ok) {
+          const int64_t off = (int64_t)mine * page_bytes + at * hs;
+          const int8_t *k = k_lane + off, *v = v_lane + off;
+          const uint32_t dst = ring + slot * S::STAGE;
 #pragma unroll
-        for (int y = 0; y < 2; y++)
+          for (int i = 0; i < HSEG * 2; i++)
+            if (WHOLE || i * 32 + lane < hs) copy<16>(dst + piece_to[i], k + i * 512);
 #pragma unroll
-          for (int j = 0; j < HSEG; j++) {
-            const bool on = ok && (WHOLE || 64 * j + 16 * c < hs);
-            copy<16>(dst + (y * HSEG + j) * 512, on || WHOLE ? k + y * 8 * hs + 64 * j : a.kc, on);
-          }
-        const uint32_t vdst = ring + slot * S::STAGE + HSEG * 1024 + lane * S::VB;
-#pragma unroll
-        for (int y = 0; y < 4; y++)
-#pragma unroll
-          for (int p = 0; p < S::VN; p++) {
-            const bool on = ok && (WHOLE || p * 8 * S::VB + S::VB * g < hs);
-            copy<S::VB>(vdst + (y * S::VN + p) * 32 * S::VB,
-                        on || WHOLE ? v + ((y & 1) + 8 * (y >> 1)) * hs + p * 8 * S::VB : a.vc, on);
-          }
+          for (int i = 0; i < HSEG * 2; i++)
+            if (WHOLE || i * 32 + lane < hs) copy<16>(dst + UNIT * S::ROW + piece_to[i], v + i * 512);
+        }
         // a table entry that is no block of the pool: NaN scales, so every row that sees it comes out NaN
         if (lane < 2) {
           float *dst_s = &sm.sc[warp][slot][lane];
-          if (ok) copy<4>(smem_addr(dst_s), s_lane + (int64_t)mine * a.nkv, true);
+          if (ok) copy<4>(smem_addr(dst_s), s_lane + (int64_t)mine * a.nkv);
           else *dst_s = __uint_as_float(0x7fffffffu);
         }
       }
       copies_commit();
     };
-    {
+    // raw scores of the unit in a slot: S^T = K Q^T, 16 positions x 8 columns an instruction
+    auto score = [&](int slot, int (&si)[S::CT][4]) {
+#pragma unroll
+      for (int t = 0; t < S::CT; t++) si[t][0] = si[t][1] = si[t][2] = si[t][3] = 0;
+      const uint8_t *base = ring_p + slot * S::STAGE;
+#pragma unroll
+      for (int j = 0; j < HSEG; j++) {
+        const uint8_t *row = base + (j >> 1) * 128 + (k_from ^ ((j & 1) << 6));
+        const uint4 k0 = *reinterpret_cast<const uint4 *>(row);
+        const uint4 k1 = *reinterpret_cast<const uint4 *>(row + 8 * S::ROW);
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+#pragma unroll
+          for (int t = 0; t < S::CT; t++) {
+            const int k = (2 * j + w) * S::CT + t;
+            uint2 q;
+            if (S::QREG) q = make_uint2(qd[S::QREG ? k : 0][0], qd[S::QREG ? k : 0][1]);
+            else q = sm.qf[S::QREG ? 0 : k * 32 + lane];
+            if (w == 0) mma_i8(si[t], k0.x, k1.x, k0.y, k1.y, q.x, q.y);
+            else mma_i8(si[t], k0.z, k1.z, k0.w, k1.w, q.x, q.y);
+          }
+      }
+    };
+    // The next unit's scores are worked out beside this unit's weights and values: neither waits for the other, and with
+    // three warps a scheduler it is waiting for one instruction after the other that takes the time.
+    if (u0 + warp < u_end) {
 #pragma unroll
       for (int s = 0; s < STAGES - 1; s++) issue(s);
+      copies_wait<STAGES - 2>();
+      __syncwarp();
+      int si[S::CT][4];
+      score(0, si);
       int slot = 0;
 #pragma unroll 1
       for (int u = u0 + warp; u < u_end; u += WARPS) {
-        copies_wait<STAGES - 2>();
-        __syncwarp();
+        const int after = slot + 1 == STAGES ? 0 : slot + 1;
+        copies_wait<STAGES - 3>();
+        __syncwarp();  // (every lane is through with the slot before this one, which is refilled at once)
+        issue(slot == 0 ? STAGES - 1 : slot - 1);
         const float kscale = sm.sc[warp][slot][0], vscale = sm.sc[warp][slot][1];
-        // ---- scores: S^T = K Q^T, 16 positions x 8 rows an instruction tile (the two parts' sums apart: the
-        // instructions of one wait for one another)
-        float s[NT][4], s_lo[NT][4];
+        const uint8_t *base = ring_p + slot * S::STAGE;
+        int next[S::CT][4];
+        score(after, next);  // (of the last unit: of what the slot held, for nothing)
+        float s[NT][4];
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) s[t][e] = s_lo[t][e] = 0.0f;
-        const uint8_t *base = ring_p + slot * S::STAGE;
-#pragma unroll
-        for (int j = 0; j < HSEG; j++) {
-          const uint4 k0 = *reinterpret_cast<const uint4 *>(base + j * 512 + lane * 16);
-          const uint4 k1 = *reinterpret_cast<const uint4 *>(base + (HSEG + j) * 512 + lane * 16);
-          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-#pragma unroll
-          for (int w = 0; w < 4; w++) {
-            const uint32_t y0 = w0[w] ^ 0x80808080u, y1 = w1[w] ^ 0x80808080u;
-            const uint32_t a0 = widen<0x4140>(y0), a1 = widen<0x4140>(y1), a2 = widen<0x4342>(y0), a3 = widen<0x4342>(y1);
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-              const int k = (4 * j + w) * NT + t;
-              if (S::QREG) {
-                // (one part: even and odd steps' sums apart)
-                mma(!PAIR && (w & 1) ? s_lo[t] : s[t], a0, a1, a2, a3, qh[S::QREG ? k : 0][0], qh[S::QREG ? k : 0][1]);
-                if (PAIR) mma(s_lo[t], a0, a1, a2, a3, ql[S::QREG && PAIR ? k : 0][0], ql[S::QREG && PAIR ? k : 0][1]);
-              } else {
-                const uint4 f = sm.qf[S::QREG ? 0 : k * 32 + lane];
-                mma(!PAIR && (w & 1) ? s_lo[t] : s[t], a0, a1, a2, a3, f.x, f.y);
-                if (PAIR) mma(s_lo[t], a0, a1, a2, a3, f.z, f.w);
-              }
+          for (int e = 0; e < 4; e++) {
+            if (BOTH) {
+              // lanes c < 2 have the first digits and the last ones, c >= 2 the second ones, of the same rows
+              const float v = (float)si[0][e] * (c < 2 ? 65536.0f : 256.0f) + (float)si[S::CT - 1][e];
+              s[t][e] = v + __shfl_xor_sync(0xffffffffu, v, 2);
+            } else {
+              s[t][e] = __fmaf_rn((float)si[t][e], 65536.0f, __fmaf_rn((float)si[(NT + t) % S::CT][e], 256.0f, (float)si[(2 * NT + t) % S::CT][e]));
             }
           }
-        }
         // ---- weights. A value scale below 2^-100 counts as 2^-100 (a block of zeros has scale 0): what it weighs
         // is below any other block's last place
         const float vs = !(vscale < LEAST) ? vscale : LEAST;
@@ -399,13 +446,11 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
           for (int p = 0; p < 2; p++) f[t][p] = kscale * qf[t][p];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            s[t][e] += s_lo[t][e];
-            if (BOTH) s[t][e] += __shfl_xor_sync(0xffffffffu, s[t][e], 2);  // the other part's sum
             y[t][e] = __fmaf_rn(s[t][e], f[t][e & 1], lg);
           }
         }
         const bool masked = u * UNIT + UNIT - 1 > first;
-        auto sees = [&](int t, int e) { return u * UNIT + g + 8 * (e >> 1) <= pos[t][e & 1]; };
+        auto sees = [&](int t, int e) { return u * UNIT + place<HSEG>(g) + 8 * (e >> 1) <= pos[t][e & 1]; };
         if (masked) {
 #pragma unroll
           for (int t = 0; t < NT; t++)
@@ -460,14 +505,16 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
             if (PAIR) pl[t][x] = transposed(lo);
           }
         }
-        // ---- O^T += V^T P^T: lane (g, c)'s pieces of the rows of positions 2c, 2c + 1, 2c + 8, 2c + 9
-        const uint8_t *vbase = base + HSEG * 1024 + lane * S::VB;
+        // ---- O^T += V^T P^T: lane (g, c)'s pieces of the rows place(2 c), place(2 c + 1), and 8 on
+        const uint8_t *vbase = base + UNIT * S::ROW;
 #pragma unroll
         for (int p = 0; p < S::VN; p++) {
           uint32_t vw[4][S::VB / 4];
 #pragma unroll
           for (int y = 0; y < 4; y++) {
-            const uint8_t *src = vbase + (y * S::VN + p) * 32 * S::VB;
+            // piece (8 p + g) of 16 bytes, or 8 bytes 8 p + g
+            const uint8_t *src = vbase + (y >> 1) * 8 * S::ROW +
+                                 (S::VB == 16 ? p * 128 + v_from[y & 1] : (p >> 1) * 128 + (v_from[y & 1] ^ ((p & 1) << 6)));
             if (S::VB == 16) {
               const uint4 v = *reinterpret_cast<const uint4 *>(src);
               vw[y][0] = v.x, vw[y][1] = v.y, vw[y][S::VB / 4 - 2] = v.z, vw[y][S::VB / 4 - 1] = v.w;
@@ -497,9 +544,11 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
             }
           }
         }
-        __syncwarp();  // every lane has read the slot's scales
-        issue(slot == 0 ? STAGES - 1 : slot - 1);
-        slot = slot + 1 == STAGES ? 0 : slot + 1;
+#pragma unroll
+        for (int t = 0; t < S::CT; t++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) si[t][e] = next[t][e];
+        slot = after;
       }
       copies_wait<0>();
     }
