@@ -32,6 +32,7 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int MOST_BLOCKS = 148 * 3;  // thread blocks of a grid (resident at once)
+constexpr int MIN_UNITS = 32;         // a span's units at least
 
 // Where a row's 16-byte piece q sits in the ring: 128-byte lines (of two rows of 64) with the pieces swapped by the row.
 // The keys' reads take pieces 4 j + c of rows place(g), g = 2 i and 2 i + 1 at a time, the values' 16 (8) bytes g of rows
@@ -102,22 +103,22 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return y;
 }
 
-// sums of {work units, tiles} over the requests before this thread's (one request a thread), and of all
-__device__ __forceinline__ void block_scan(int64_t (&v)[2], int64_t (&all)[2], int64_t (*part)[WARPS]) {
+// sums of {work, tiles, new tokens} over the requests before this thread's (one request a thread), and of all
+__device__ __forceinline__ void block_scan(int64_t (&v)[3], int64_t (&all)[3], int64_t (*part)[WARPS]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t own[2] = {v[0], v[1]};
+  const int64_t own[3] = {v[0], v[1], v[2]};
 #pragma unroll
-  for (int j = 0; j < 2; j++)
+  for (int j = 0; j < 3; j++)
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int64_t o = __shfl_up_sync(0xffffffffu, v[j], d);
       if (lane >= d) v[j] += o;
     }
   __syncthreads();
-  if (lane == 31) part[0][warp] = v[0], part[1][warp] = v[1];
+  if (lane == 31) part[0][warp] = v[0], part[1][warp] = v[1], part[2][warp] = v[2];
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
+  for (int j = 0; j < 3; j++) {
     all[j] = 0;
     int64_t before = 0;
 #pragma unroll
@@ -152,7 +153,7 @@ struct Shape {
     alignas(16) uint2 qf[QREG ? 1 : KSTEPS * CT * 32];
     float sc[WARPS][STAGES][2];                     // the units' scales
     float ml[WARPS][RT][2];
-    int64_t part[2][WARPS];
+    int64_t part[3][WARPS];
     int64_t found[3];
   };
 };
@@ -170,55 +171,46 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int h = blockIdx.y;
 
-  // ---- this block's span of the units
-  int64_t total = 0, fresh = 0;
-  for (int i = tid; i < a.n_seqs; i += THREADS) {
-    const Request r = request_of(a, i);
-    fresh += r.fresh;
-    total += (int64_t)tiles_of<RT>(a, r) * units_of(a, r);
-  }
+  // ---- this block's span of the work, and the request in which it begins; {work, tiles} before that request. Work is
+  // units, or, where no tile is longer than a span has to be, tiles (none is cut then).
+  int64_t before[2] = {0, 0};
+  int64_t v[3], all[3], sum[3] = {0, 0, 0}, w = 0;
+  auto add_up = [&](int base) {
+    const int i = base + tid;
+    v[0] = v[1] = v[2] = w = 0;
+    if (i < a.n_seqs) {
+      const Request r = request_of(a, i);
+      v[2] = r.fresh;
+      v[1] = tiles_of<RT>(a, r);
+      w = v[0] = v[1] * (a.whole_tiles ? 1 : units_of(a, r));
+    }
+    block_scan(v, all, sm.part);
+  };
+  for (int base = 0; base < a.n_seqs; base += THREADS) {
+    add_up(base);
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, d);
-    fresh += __shfl_xor_sync(0xffffffffu, fresh, d);
+    for (int j = 0; j < 3; j++) sum[j] += all[j];
   }
-  if (lane == 0) sm.part[0][warp] = total, sm.part[1][warp] = fresh;
-  __syncthreads();
-  total = sm.part[0][0] + sm.part[0][1] + sm.part[0][2] + sm.part[0][3];
-  fresh = sm.part[1][0] + sm.part[1][1] + sm.part[1][2] + sm.part[1][3];
-  if (fresh > a.n) total = 0;  // starts that don't ascend: rows of several requests, nothing is written
-  const int64_t span = max((int64_t)a.min_units, (total + gridDim.x - 1) / gridDim.x);
+  // (starts that don't ascend: rows of several requests, nothing is written)
+  const int64_t total = sum[2] > a.n ? 0 : sum[0];
+  const int64_t span = max((int64_t)a.min_work, (total + gridDim.x - 1) / gridDim.x);
   int64_t at = span * blockIdx.x;
   const int64_t end = min(at + span, total);
-  if (at >= end) {
-    if (total == 0 && blockIdx.x == 0 && h == 0 && tid == 0) a.meta[-1] = make_int4(0, 0, 0, 0);
-    return;
-  }
-  // ---- the request in which it begins; {units, tiles} before that request
-  int64_t before[2] = {0, 0};
-  int req = 0;
-  {
-    int64_t carry[2] = {0, 0};
-    for (int base = 0; base < a.n_seqs; base += THREADS) {
-      const int i = base + tid;
-      int64_t v[2] = {0, 0}, all[2], w = 0;
-      if (i < a.n_seqs) {
-        const Request r = request_of(a, i);
-        v[1] = tiles_of<RT>(a, r);
-        w = v[0] = v[1] * units_of(a, r);
-      }
-      block_scan(v, all, sm.part);
-      if (w && carry[0] + v[0] <= at && at < carry[0] + v[0] + w) {
-        sm.found[0] = carry[0] + v[0];
-        sm.found[1] = carry[1] + v[1];
-        sm.found[2] = i;
-      }
-      carry[0] += all[0], carry[1] += all[1];
+  if (blockIdx.x == 0 && h == 0 && tid == 0) a.meta[-1] = make_int4(total ? (int)sum[1] : 0, 0, 0, 0);
+  if (at >= end) return;
+  int64_t carry[2] = {0, 0};
+  for (int base = 0; base < a.n_seqs; base += THREADS) {
+    if (a.n_seqs > THREADS) add_up(base);
+    if (w && carry[0] + v[0] <= at && at < carry[0] + v[0] + w) {
+      sm.found[0] = carry[0] + v[0];
+      sm.found[1] = carry[1] + v[1];
+      sm.found[2] = base + tid;
     }
-    __syncthreads();
-    before[0] = sm.found[0], before[1] = sm.found[1], req = (int)sm.found[2];
-    if (blockIdx.x == 0 && h == 0 && tid == 0) a.meta[-1] = make_int4((int)carry[1], 0, 0, 0);
+    carry[0] += all[0], carry[1] += all[1];
   }
+  __syncthreads();
+  before[0] = sm.found[0], before[1] = sm.found[1];
+  int req = (int)sm.found[2];
 
   const int page_bytes = a.nkv * a.block * hs;
   const int step_blocks = WARPS * UNIT / a.block, step_rest = WARPS * UNIT % a.block;  // a warp's way to its next unit
@@ -231,12 +223,14 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
       req++;
       continue;
     }
-    const int tile = (int)((at - before[0]) / units), u0 = (int)((at - before[0]) % units);
-    const int u1 = (int)min((int64_t)units, u0 + (end - at));
-    const int64_t tile_at = before[0] + (int64_t)tile * units;
-    const int span0 = (int)(tile_at / span), spans = (int)((tile_at + units - 1) / span) - span0 + 1;
+    const int per_tile = a.whole_tiles ? 1 : units;
+    const int tile = (int)((at - before[0]) / per_tile), begin = (int)((at - before[0]) % per_tile);
+    const int stop = (int)min((int64_t)per_tile, begin + (end - at));
+    const int u0 = begin, u1 = a.whole_tiles ? units : stop;
+    const int64_t tile_at = before[0] + (int64_t)tile * per_tile;
+    const int span0 = (int)(tile_at / span), spans = (int)((tile_at + per_tile - 1) / span) - span0 + 1;
     const int64_t tile_id = before[1] + tile;
-    if (h == 0 && tid == 0 && u0 == 0) a.meta[tile_id] = make_int4(span0, spans, req, tile);
+    if (h == 0 && tid == 0 && begin == 0) a.meta[tile_id] = make_int4(span0, spans, req, tile);
 
     // ---- the tile's rows: row x is query head x % group of the kv head, of the request's token x / group
     const int rows = r.fresh * a.group, x0 = tile * RT, cap = a.width * a.block;
@@ -244,13 +238,68 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
     const int first = r.length - r.fresh + x0 / a.group;                       // the first row's
     const int u_end = min(u1, (min(last + 1, cap) + UNIT - 1) / UNIT);         // no row sees further units
 
+    // this lane's places in the ring: of the pieces it copies, and of those it multiplies (of the first half of the rows)
+    int piece_to[HSEG * 2];
+#pragma unroll
+    for (int i = 0; i < HSEG * 2; i++) {
+      const int piece = i * 32 + lane, per = WHOLE ? HSEG * 4 : hs / 16;
+      piece_to[i] = piece_at<HSEG>(piece / per, piece % per);
+    }
+    const int k_from = piece_at<HSEG>(place<HSEG>(g), c);
+    const int v_from[2] = {piece_at<HSEG>(place<HSEG>(2 * c), S::VB == 16 ? g : g >> 1) + (S::VB == 16 ? 0 : (g & 1) * 8),
+                           piece_at<HSEG>(place<HSEG>(2 * c + 1), S::VB == 16 ? g : g >> 1) + (S::VB == 16 ? 0 : (g & 1) * 8)};
+    // The ring's front: the next unit to copy, its block's place in the table and its place in the block, and the id of
+    // that block (read one unit ahead).
+    const int32_t *table = a.tables + (int64_t)req * a.width;
+    int front = u0 + warp, front_block = front * UNIT / a.block, front_at = front * UNIT % a.block;
+    auto forward = [&]() {
+      front += WARPS;
+      front_block += step_blocks, front_at += step_rest;
+      if (front_at >= a.block) front_at -= a.block, front_block++;
+    };
+    auto front_page = [&]() { return front < u_end ? table[front_block] : -1; };
+    // (the first units' at once: a lane a unit)
+    const int ids = front + lane * WARPS < u_end && lane < STAGES ? table[(front + lane * WARPS) * UNIT / a.block] : -1;
+    int page = __shfl_sync(0xffffffffu, ids, 0);
+    const int8_t *k_lane = a.kc + (int64_t)h * a.block * hs + lane * 16;
+    const int8_t *v_lane = a.vc + (int64_t)h * a.block * hs + lane * 16;
+    const float *s_lane = (lane == 1 ? a.vs : a.ks) + h;
+    auto issue = [&](int slot, auto &&next_page) {
+      const int mine = page, at = front_at;
+      const bool there = front < u_end, ok = (uint32_t)mine < (uint32_t)a.blocks;
+      forward();
+      page = next_page();
+      if (there) {
+        if (ok) {
+          const int64_t off = (int64_t)mine * page_bytes + at * hs;
+          const int8_t *k = k_lane + off, *v = v_lane + off;
+          const uint32_t dst = ring + slot * S::STAGE;
+#pragma unroll
+          for (int i = 0; i < HSEG * 2; i++)
+            if (WHOLE || i * 32 + lane < hs) copy<16>(dst + piece_to[i], k + i * 512);
+#pragma unroll
+          for (int i = 0; i < HSEG * 2; i++)
+            if (WHOLE || i * 32 + lane < hs) copy<16>(dst + UNIT * S::ROW + piece_to[i], v + i * 512);
+        }
+        // a table entry that is no block of the pool: NaN scales, so every row that sees it comes out NaN
+        if (lane < 2) {
+          float *dst_s = &sm.sc[warp][slot][lane];
+          if (ok) copy<4>(smem_addr(dst_s), s_lane + (int64_t)mine * a.nkv);
+          else *dst_s = __uint_as_float(0x7fffffffu);
+        }
+      }
+      copies_commit();
+    };
+    __syncthreads();  // (the tile before has left the ring)
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; s++) issue(s, [&]() { return __shfl_sync(0xffffffffu, ids, s + 1); });
+
     // this lane's column p of row tile t, as a row of the tile
     auto row_of = [&](int t, int p) { return BOTH ? 2 * (c & 1) + p : 8 * t + 2 * c + p; };
     // Query fragments: lane (g, c) holds column 8 t + g of column tile t, digit (8 t + g) / RT of row (8 t + g) % RT, of the
     // head's values 64 j + 16 c .. + 15, the bytes of keys that it copies.
     uint32_t qd[S::QREG ? S::KSTEPS * S::CT : 1][2];
     float qf[NT][2];  // what the scores of this lane's columns (rows 2 c, 2 c + 1 of row tile t) are to be scaled by
-    __syncthreads();
     {
       float f[NT], back[NT];
       int64_t off[NT];
@@ -282,32 +331,39 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
         qf[t][0] = __shfl_sync(0xffffffffu, back[t], BOTH ? 8 * (c & 1) : 8 * c) * a.scale;
         qf[t][1] = __shfl_sync(0xffffffffu, back[t], BOTH ? 8 * (c & 1) + 4 : 8 * c + 4) * a.scale;
       }
+      auto keep = [&](int k, uint32_t first, uint32_t then) {
+        if (S::QREG) qd[S::QREG ? k : 0][0] = first, qd[S::QREG ? k : 0][1] = then;
+        else if (warp == 0) sm.qf[S::QREG ? 0 : k * 32 + lane] = make_uint2(first, then);
+      };
 #pragma unroll
-      for (int t = 0; t < S::CT; t++) {
-        const int row_tile = BOTH ? 0 : t % NT, digit = BOTH ? 2 * t + (g >> 2) : t / NT;
+      for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int i = 0; i < S::KSTEPS; i++) {
-          uint32_t word[2] = {0, 0};
+          uint32_t word[3][2] = {};
           const int d = 64 * (i / 2) + 16 * c + 8 * (i & 1);
-          if (is[row_tile] && digit < 3 && (WHOLE || d < hs)) {
+          if (is[t] && (WHOLE || d < hs)) {
 #pragma unroll
             for (int y = 0; y < 2; y++) {
               float z[4];
-              query<HALF>(a.q, off[row_tile] + d + 4 * y, z);
+              query<HALF>(a.q, off[t] + d + 4 * y, z);
 #pragma unroll
               for (int e = 0; e < 4; e++) {
-                // q 2^21 = 65536 d0 + 256 d1 + d2, the digits from -128 to 127
-                const int whole = __float2int_rn(z[e] * f[row_tile] * 2097152.0f);
-                const int d2 = (int8_t)whole, upper = (whole - d2) >> 8, d1 = (int8_t)upper, d0 = (upper - d1) >> 8;
-                word[y] |= (uint32_t)((digit == 0 ? d0 : digit == 1 ? d1 : d2) & 255) << (8 * e);
+                // q 2^21 = 65536 d0 + 256 d1 + d2, the digits from -128 to 127: with 128 added to the lower two, the
+                // bytes of the sum, less that
+                const uint32_t sum = (uint32_t)(__float2int_rn(z[e] * f[t] * 2097152.0f) + 0x8080) ^ 0x8080u;
+#pragma unroll
+                for (int k = 0; k < 3; k++) word[k][y] |= (sum >> (16 - 8 * k) & 255) << (8 * e);
               }
             }
           }
-          const int k = i * S::CT + t;
-          if (S::QREG) qd[S::QREG ? k : 0][0] = word[0], qd[S::QREG ? k : 0][1] = word[1];
-          else if (warp == 0) sm.qf[S::QREG ? 0 : k * 32 + lane] = make_uint2(word[0], word[1]);
+          if (BOTH) {
+            keep(i * S::CT, g < 4 ? word[0][0] : word[1][0], g < 4 ? word[0][1] : word[1][1]);
+            keep(i * S::CT + S::CT - 1, g < 4 ? word[2][0] : 0, g < 4 ? word[2][1] : 0);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 3; k++) keep((i * S::CT + k * NT + t) % (S::KSTEPS * S::CT), word[k][0], word[k][1]);
+          }
         }
-      }
     }
     int pos[NT][2];  // the positions of this lane's columns (-1: no row)
 #pragma unroll
@@ -328,56 +384,6 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
 #pragma unroll
       for (int m = 0; m < HSEG * 4; m++) o[t][m][0] = o[t][m][1] = o[t][m][2] = o[t][m][3] = 0.0f;
     }
-    // this lane's places in the ring: of the pieces it copies, and of those it multiplies (of the first half of the rows)
-    int piece_to[HSEG * 2];
-#pragma unroll
-    for (int i = 0; i < HSEG * 2; i++) {
-      const int piece = i * 32 + lane, per = WHOLE ? HSEG * 4 : hs / 16;
-      piece_to[i] = piece_at<HSEG>(piece / per, piece % per);
-    }
-    const int k_from = piece_at<HSEG>(place<HSEG>(g), c);
-    const int v_from[2] = {piece_at<HSEG>(place<HSEG>(2 * c), S::VB == 16 ? g : g >> 1) + (S::VB == 16 ? 0 : (g & 1) * 8),
-                           piece_at<HSEG>(place<HSEG>(2 * c + 1), S::VB == 16 ? g : g >> 1) + (S::VB == 16 ? 0 : (g & 1) * 8)};
-    // The ring's front: the next unit to copy, its block's place in the table and its place in the block, and the id of
-    // that block (read one unit ahead).
-    const int32_t *table = a.tables + (int64_t)req * a.width;
-    int front = u0 + warp, front_block = front * UNIT / a.block, front_at = front * UNIT % a.block;
-    auto forward = [&]() {
-      front += WARPS;
-      front_block += step_blocks, front_at += step_rest;
-      if (front_at >= a.block) front_at -= a.block, front_block++;
-    };
-    auto front_page = [&]() { return front < u_end ? table[front_block] : -1; };
-    int page = front_page();
-    const int8_t *k_lane = a.kc + (int64_t)h * a.block * hs + lane * 16;
-    const int8_t *v_lane = a.vc + (int64_t)h * a.block * hs + lane * 16;
-    const float *s_lane = (lane == 1 ? a.vs : a.ks) + h;
-    auto issue = [&](int slot) {
-      const int mine = page, at = front_at;
-      const bool there = front < u_end, ok = (uint32_t)mine < (uint32_t)a.blocks;
-      forward();
-      page = front_page();
-      if (there) {
-        if (ok) {
-          const int64_t off = (int64_t)mine * page_bytes + at * hs;
-          const int8_t *k = k_lane + off, *v = v_lane + off;
-          const uint32_t dst = ring + slot * S::STAGE;
-#pragma unroll
-          for (int i = 0; i < HSEG * 2; i++)
-            if (WHOLE || i * 32 + lane < hs) copy<16>(dst + piece_to[i], k + i * 512);
-#pragma unroll
-          for (int i = 0; i < HSEG * 2; i++)
-            if (WHOLE || i * 32 + lane < hs) copy<16>(dst + UNIT * S::ROW + piece_to[i], v + i * 512);
-        }
-        // a table entry that is no block of the pool: NaN scales, so every row that sees it comes out NaN
-        if (lane < 2) {
-          float *dst_s = &sm.sc[warp][slot][lane];
-          if (ok) copy<4>(smem_addr(dst_s), s_lane + (int64_t)mine * a.nkv);
-          else *dst_s = __uint_as_float(0x7fffffffu);
-        }
-      }
-      copies_commit();
-    };
     // raw scores of the unit in a slot: S^T = K Q^T, 16 positions x 8 columns an instruction
     auto score = [&](int slot, int (&si)[S::CT][4]) {
 #pragma unroll
@@ -404,8 +410,6 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
     // The next unit's scores are worked out beside this unit's weights and values: neither waits for the other, and with
     // three warps a scheduler it is waiting for one instruction after the other that takes the time.
     if (u0 + warp < u_end) {
-#pragma unroll
-      for (int s = 0; s < STAGES - 1; s++) issue(s);
       copies_wait<STAGES - 2>();
       __syncwarp();
       int si[S::CT][4];
@@ -416,7 +420,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
         const int after = slot + 1 == STAGES ? 0 : slot + 1;
         copies_wait<STAGES - 3>();
         __syncwarp();  // (every lane is through with the slot before this one, which is refilled at once)
-        issue(slot == 0 ? STAGES - 1 : slot - 1);
+        issue(slot == 0 ? STAGES - 1 : slot - 1, front_page);
         const float kscale = sm.sc[warp][slot][0], vscale = sm.sc[warp][slot][1];
         const uint8_t *base = ring_p + slot * S::STAGE;
         int next[S::CT][4];
@@ -550,8 +554,8 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
           for (int e = 0; e < 4; e++) si[t][e] = next[t][e];
         slot = after;
       }
-      copies_wait<0>();
     }
+    copies_wait<0>();
 
     // ---- the four warps' sums to one M a row, then added in the warps' order
 #pragma unroll
@@ -624,9 +628,9 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
         if (d == 0) a.part_ml[row] = make_float2(top, sum_l);
       }
     }
-    at += u1 - u0;
-    if (tile + 1 == tiles && u1 == units) {
-      before[0] += (int64_t)tiles * units;
+    at += stop - begin;
+    if (tile + 1 == tiles && stop == per_tile) {
+      before[0] += (int64_t)tiles * per_tile;
       before[1] += tiles;
       req++;
     }
@@ -755,7 +759,7 @@ int launch_attention8(const Args &a, int blocks_x, cudaStream_t stream) {
   using S = Shape<HSEG, RT, HALF>;
   auto kernel = cache8_attention_kernel<HSEG, RT, HALF, WHOLE>;
   B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename S::Smem)));
-  const int most = 148 * S::MINB / a.nkv;
+  const int most = a.whole_tiles ? blocks_x : 148 * S::MINB / a.nkv;
   launch(kernel, dim3(most < 1 ? 1 : most < blocks_x ? most : blocks_x, a.nkv), dim3(THREADS), sizeof(typename S::Smem),
          stream, a);
   B200_LAUNCHED("cache8_attention");
@@ -830,10 +834,12 @@ extern "C" int b200k_cache8_attention(void *out, const void *q, const int8_t *kc
     // blocks of tokens go to the tensor cores; where there is no more than a token a request on average, any request is
     // taken here, and one kernel less launched
     const bool prompts = n > n_seqs && prompts_fit(hs);
+    // tables of no more positions than a span has: a thread block a tile, and nothing to join
+    const bool whole_tiles = (int64_t)table_width * block <= MIN_UNITS * UNIT;
     Args a = {out, q, kc, vc, ks, vs, tables, starts, lengths, reinterpret_cast<int4 *>(base) + 1,
               reinterpret_cast<float2 *>(base + s.ml_at), reinterpret_cast<float *>(base + s.part_at), q_stride,
-              out_stride, n, n_seqs, table_width, blocks, block, nkv, hs, nh / nkv, 8,
-              prompts ? ROWS_FEW : INT32_MAX,
+              out_stride, n, n_seqs, table_width, blocks, block, nkv, hs, nh / nkv,
+              whole_tiles ? 1 : MIN_UNITS, whole_tiles, prompts ? ROWS_FEW : INT32_MAX,
               1.4426950408889634f / sqrtf((float)hs)};
     const cudaStream_t st = as_stream(stream);
     const int hseg = (hs + 63) / 64, blocks_x = (MOST_BLOCKS + nkv - 1) / nkv;
@@ -842,9 +848,9 @@ extern "C" int b200k_cache8_attention(void *out, const void *q, const int8_t *kc
                                 : hseg == 2 ? launch_of<2>(s.rt, half, whole)
                                 : hseg == 3 ? launch_of<3>(s.rt, half, whole)
                                             : launch_of<4>(s.rt, half, whole);
-    rc = launch_units(a, blocks_x, st);
+    rc = launch_units(a, whole_tiles ? (int)(s.tiles < 65535 ? s.tiles : 65535) : blocks_x, st);
     if (!rc && prompts) rc = launch_attention8_prompts(a, half, st);
-    if (rc) return rc;
+    if (rc || whole_tiles) return rc;
     return s.rt == 4   ? launch_combine<4, false>(a, s.tiles, st)
            : s.rt == 8 ? (half ? launch_combine<8, true>(a, s.tiles, st) : launch_combine<8, false>(a, s.tiles, st))
                        : (half ? launch_combine<16, true>(a, s.tiles, st) : launch_combine<16, false>(a, s.tiles, st));

@@ -25,7 +25,8 @@ struct Args {
   float2 *part_ml;  // [span + tile][kv head][RT] {M, l}
   float *part;      // [span + tile][kv head][RT][hs]
   int64_t q_stride, out_stride;
-  int n, n_seqs, width, blocks, block, nkv, hs, group, min_units;
+  int n, n_seqs, width, blocks, block, nkv, hs, group;
+  int min_work, whole_tiles;  // a span's work at least, in units or (whole_tiles) in tiles
   int rows_most;       // a request's rows of a kv head above which it is not cache8_attention.cu's
   float scale;      // log2(e) / sqrt(hs)
 };
