@@ -310,6 +310,7 @@ int b200k_attention_batch(float *out, const float *q, const void *kc, const void
  * tokens are rows starts[i]..starts[i + 1] - 1; slots, seq and pos [n], each token's slot, request and position (seq and
  * pos may be NULL), -1 in rows behind the last token. lengths_out may be lengths and state_out state (updated in
  * place); no other two arrays may overlap.
+ * Up to 2^20 requests and 2^30 tokens, table_width * block up to 2^30.
  * All or nothing: where the status is not 0, lengths, tables, ring, head and count stay, and the step has no tokens. */
 #define B200K_TABLES_BLOCKS 1 /* too few free blocks */
 #define B200K_TABLES_TOKENS 2 /* more than n tokens */

@@ -16,6 +16,14 @@
 namespace b200 {
 namespace {
 
+// x / by for 0 <= x < 2^31 and by from 16 to 256, inverse = ceil(2^32 / by): the product is never below the quotient, and
+// one above at most
+__host__ __device__ inline uint32_t inverse_of(int by) { return 0xffffffffu / (uint32_t)by + 1; }
+__device__ __forceinline__ int over(int x, int by, uint32_t inverse) {
+  const int q = (int)__umulhi((uint32_t)x, inverse);
+  return (uint32_t)q * (uint32_t)by > (uint32_t)x ? q - 1 : q;
+}
+
 // ------------------------------------------------------------------------------------------------ block tables
 //
 // L' = max(0, L + news) positions a request: its blocks go from ceil(L / block) to ceil(L' / block), new ones taken
@@ -79,102 +87,111 @@ struct TablesArgs {
 __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
   pdl_begin();
   __shared__ int64_t part[3][TT / 32];
-  __shared__ int bad_s, sums[3][TT + 1], len_s[TT];
+  __shared__ int sums[3][TT + 1], len_s[TT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t rank, ranks;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   const int64_t most = (int64_t)a.width * a.block;
-  if (tid == 0) bad_s = 0;
-  __syncthreads();
+  const int head = a.state[0], count = a.state[1];
+  const uint32_t inverse = inverse_of(a.block);
+  auto over_block = [&](int x) { return over(x, a.block, inverse); };
+
+  // this thread's request of a tile, what it needs, and the sums of that before it and over the tile
+  int length = 0, bad = 0;
+  int64_t after = 0, run[3], all[3];
+  Need need = {0, 0, 0};
+  auto tile_of = [&](int base) {
+    const int i = base + tid;
+    need = {0, 0, 0};
+    length = 0;
+    if (i < a.n_seqs) {
+      length = a.lengths[i];
+      need = need_of(length, a.news[i], most, a.block, bad, after);
+    }
+    const int64_t own[3] = {need.tokens, need.take, need.give};
+#pragma unroll
+    for (int j = 0; j < 3; j++) run[j] = warp_scan(own[j]);
+    __syncthreads();  // (the tile before has been read)
+    if (lane == 31) part[0][warp] = run[0], part[1][warp] = run[1], part[2][warp] = run[2];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 3; j++) {
+      int64_t before = 0;
+      all[j] = 0;
+#pragma unroll
+      for (int w = 0; w < TT / 32; w++) {
+        if (w < warp) before += part[j][w];
+        all[j] += part[j][w];
+      }
+      run[j] += before - own[j];
+    }
+  };
 
   // what everything comes to: all is granted, or nothing is
   int64_t sum[3] = {0, 0, 0};
-  int bad = 0;
-  for (int i = tid; i < a.n_seqs; i += TT) {
-    int64_t after;
-    const Need w = need_of(a.lengths[i], a.news[i], most, a.block, bad, after);
-    sum[0] += w.tokens;
-    sum[1] += w.take;
-    sum[2] += w.give;
-  }
+  for (int base = 0; base < a.n_seqs; base += TT) {
+    tile_of(base);
 #pragma unroll
-  for (int j = 0; j < 3; j++) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], d);
-    if (lane == 0) part[j][warp] = sum[j];
+    for (int j = 0; j < 3; j++) sum[j] += all[j];
   }
-  if (bad) atomicOr(&bad_s, bad);
-  const int head = a.state[0], count = a.state[1];
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < 3; j++) {
-    sum[j] = 0;
-    for (int w = 0; w < TT / 32; w++) sum[j] += part[j][w];
-  }
-  bad = bad_s;
+  bad = __syncthreads_or(bad & 1 << B200K_TABLES_INPUT) ? 1 << B200K_TABLES_INPUT
+        : __syncthreads_or(bad & 1 << B200K_TABLES_WIDTH) ? 1 << B200K_TABLES_WIDTH : 0;
   if (head < 0 || head >= a.blocks || count < 0 || count > a.blocks || count + sum[2] > a.blocks)
-    bad |= 1 << B200K_TABLES_INPUT;
+    bad = 1 << B200K_TABLES_INPUT;
   if (sum[0] > a.n) bad |= 1 << B200K_TABLES_TOKENS;
   if (sum[1] > count) bad |= 1 << B200K_TABLES_BLOCKS;
   const bool granted = bad == 0;
   const int total = granted ? (int)sum[0] : 0;
+  auto in_ring = [&](int u) {  // the ring's place u after its head, u below 2^31 - blocks
+    const int at = head + u;
+    return at >= a.blocks ? at - a.blocks : at;
+  };
 
   const int stride = (int)ranks * TT, first = (int)rank * TT + tid;
   int carry[3] = {0, 0, 0};
   if (granted) {
     for (int base = 0; base < a.n_seqs; base += TT) {
-      const int i = base + tid, tile = min(TT, a.n_seqs - base);
-      Need w = {0, 0, 0};
-      int length = 0;
-      if (i < a.n_seqs) {
-        int64_t after;
-        int none = 0;
-        length = a.lengths[i];
-        w = need_of(length, a.news[i], most, a.block, none, after);
-      }
-      int64_t run[3] = {w.tokens, w.take, w.give};
-      __syncthreads();  // the tile before has been read
-#pragma unroll
-      for (int j = 0; j < 3; j++) {
-        run[j] = warp_scan(run[j]);
-        if (lane == 31) part[j][warp] = run[j];
-      }
+      const int tile = min(TT, a.n_seqs - base);
+      if (a.n_seqs > TT) tile_of(base);
       len_s[tid] = length;
-      __syncthreads();
-      const int64_t own[3] = {w.tokens, w.take, w.give};
 #pragma unroll
       for (int j = 0; j < 3; j++) {
-        int64_t before = carry[j];
-        for (int v = 0; v < warp; v++) before += part[j][v];
-        sums[j][tid] = (int)(before + run[j] - own[j]);
-        if (tid == TT - 1) sums[j][TT] = (int)(before + run[j]);
+        sums[j][tid] = (int)(carry[j] + run[j]);
+        if (tid == 0) sums[j][TT] = (int)(carry[j] + all[j]);
       }
       __syncthreads();
-      if (tid < tile && rank == 0) a.starts[i] = sums[0][tid];
-      // the tokens of this tile of requests, their slots from the table or, in blocks taken now, from the ring
-      for (int t = carry[0] + first; t < sums[0][TT]; t += stride) {
-        const int s = find(sums[0], tile, t), p = len_s[s] + (t - sums[0][s]), b = p / a.block;
-        const int held = (len_s[s] + a.block - 1) / a.block;
-        int id;
-        if (b < held) {
-          id = a.tables[(int64_t)(base + s) * a.width + b];
-        } else {
-          int64_t at = (int64_t)head + sums[1][s] + (b - held);
-          id = a.ring[at % a.blocks];
+      if (tid < tile && rank == 0) a.starts[base + tid] = sums[0][tid];
+      // the tokens of this tile of requests, their slots from the table or, in blocks taken now, from the ring; a few of
+      // them at a time, so that their lookups overlap
+      constexpr int AT_ONCE = 4;
+      for (int t0 = carry[0] + first; t0 < sums[0][TT]; t0 += AT_ONCE * stride) {
+        int s[AT_ONCE], p[AT_ONCE], id[AT_ONCE], b[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++) s[k] = find(sums[0], tile, min(t0 + k * stride, sums[0][TT] - 1));
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++) {
+          p[k] = len_s[s[k]] + (min(t0 + k * stride, sums[0][TT] - 1) - sums[0][s[k]]);
+          b[k] = over_block(p[k]);
+          const int held = over_block(len_s[s[k]] + a.block - 1);
+          id[k] = b[k] < held ? a.tables[(int64_t)(base + s[k]) * a.width + b[k]] : a.ring[in_ring(sums[1][s[k]] + (b[k] - held))];
         }
-        a.slots[t] = id >= 0 && id < a.blocks ? id * a.block + (p - b * a.block) : -1;
-        if (a.seq) a.seq[t] = base + s;
-        if (a.pos) a.pos[t] = p;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++) {
+          const int t = t0 + k * stride;
+          if (t >= sums[0][TT]) break;
+          a.slots[t] = id[k] >= 0 && id[k] < a.blocks ? id[k] * a.block + (p[k] - b[k] * a.block) : -1;
+          if (a.seq) a.seq[t] = base + s[k];
+          if (a.pos) a.pos[t] = p[k];
+        }
       }
       for (int u = carry[1] + first; u < sums[1][TT]; u += stride) {
-        const int s = find(sums[1], tile, u), held = (len_s[s] + a.block - 1) / a.block;
-        a.tables[(int64_t)(base + s) * a.width + held + (u - sums[1][s])] = a.ring[((int64_t)head + u) % a.blocks];
+        const int s = find(sums[1], tile, u), held = over_block(len_s[s] + a.block - 1);
+        a.tables[(int64_t)(base + s) * a.width + held + (u - sums[1][s])] = a.ring[in_ring(u)];
       }
       for (int u = carry[2] + first; u < sums[2][TT]; u += stride) {
-        const int s = find(sums[2], tile, u), held = (len_s[s] + a.block - 1) / a.block;
         // request s keeps its first held - (its gives) blocks
-        const int gives = sums[2][s + 1] - sums[2][s];
+        const int s = find(sums[2], tile, u), held = over_block(len_s[s] + a.block - 1), gives = sums[2][s + 1] - sums[2][s];
         a.ring[((int64_t)head + count + u) % a.blocks] =
             a.tables[(int64_t)(base + s) * a.width + held - gives + (u - sums[2][s])];
       }
@@ -195,12 +212,12 @@ __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
   if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   else __syncthreads();
   for (int i = first; i < a.n_seqs; i += stride) {
-    int64_t after = a.lengths[i];
-    if (granted) {
+    if (a.n_seqs > TT || ranks > 1) {
+      length = a.lengths[i];
       int none = 0;
-      need_of(after, a.news[i], most, a.block, none, after);
+      need_of(length, a.news[i], most, a.block, none, after);
     }
-    a.lengths_out[i] = (int)after;
+    a.lengths_out[i] = granted ? (int)after : length;
   }
   if (rank == 0 && tid == 0) {
     int status = 0;
@@ -218,15 +235,17 @@ __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
 // ------------------------------------------------------------------------------------------------------- store
 //
 // A (block, head)'s scale is s = max |x| / 127 in float32 over all that it holds, and every value is the integer
-// nearest to x / s, half to even, of the real quotient: a float32 guess, then the exact remainder decides. A token
-// that raises the scale of a block with earlier tokens in it has their integers q brought to the new step,
-// nearest(q s_old / s): one scale a block costs that, and only blocks that a request still fills pay it.
+// nearest to x / s, half to even, of the real quotient: a float32 guess, and where its remainder comes near half a step,
+// the exact one. A token that raises the scale of a block with earlier tokens in it has their integers q brought to the
+// new step, nearest(q s_old / s): one scale a block costs that, and only blocks that a request still fills pay it.
 //
 // Tokens of a block stand together in the call (a request's positions do), so the block's work belongs to the place
-// where its run of tokens begins: no two thread blocks touch one (block, head), and no atomics.
+// where its run of tokens begins: no two teams touch one (block, head), and no atomics. A team is a thread block, or a
+// warp where the call has few tokens; it keeps the values that fit its registers between finding the largest and
+// rounding (the rest it reads again, from L1).
 
-constexpr int ST = 128;  // threads
-constexpr int KEEP = 8;  // 16-byte vectors of new values that a thread keeps in registers between its two passes
+constexpr int ST = 128;  // threads of a block
+constexpr int KEEP = 4;  // 16-byte vectors of new values that a thread keeps in registers between its two passes
 
 __device__ __forceinline__ void values_of(const uint4 &u, float (&x)[4]) {
   x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
@@ -240,53 +259,57 @@ __device__ __forceinline__ void values_of(const uint4 &u, float (&x)[8]) {
   }
 }
 
-// the integer nearest to x / s (half to even), |x| <= 127 s (1 + 2^-24), inv about 1 / s
-__device__ __forceinline__ int nearest(float x, float s, float inv) {
-  float q = rintf(__fmul_rn(x, inv));
-  // x - q s is exact: a multiple of s's last place, and no larger than about s
-  const float r = __fmaf_rn(-q, s, x);
-  const float twice = __fadd_rn(fabsf(r), fabsf(r));
-  if (twice > s) {
-    q = __fadd_rn(q, r > 0 ? 1.0f : -1.0f);
-  } else if (twice == s) {
-    // halfway between q and its neighbour on r's side: the even one
-    if ((int)q & 1) q = __fadd_rn(q, r > 0 ? 1.0f : -1.0f);
-  }
-  return (int)q;
+// the integer nearest to q a / b, half to even, in 64 bits: q a is exact there (q an integer of 8 bits, or 1 and a a
+// float), and so far from a half that is not one that the quotient's rounding cannot reach it
+__device__ __noinline__ int exactly(double qa, double b) { return (int)rint(__ddiv_rn(qa, b)); }
+
+// the largest |x|: NaN above infinity above every number
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
-
-// nearest(q a / b), a <= b, in 64 bits (q a is exact there, the quotient's halves too): few values need it
-__device__ __forceinline__ int moved(int q, double a, double b) { return (int)rint(__ddiv_rn(__dmul_rn((double)q, a), b)); }
-
-// the largest |x| as its bits: NaN above infinity above every number, so the maximum keeps both
 template <int VW>
-__device__ __forceinline__ uint32_t largest_bits(const uint4 &u) {
+__device__ __forceinline__ float largest(float top, const uint4 &u) {
   float x[VW];
   values_of(u, x);
-  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < VW; i++) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-  return m;
+  for (int i = 0; i < VW; i++) top = max_nan(top, fabsf(x[i]));
+  return top;
 }
 
-template <int VW>
-__device__ __forceinline__ void put(int8_t *dst, const uint4 &u, float s, float inv) {
-  float x[VW];
-  values_of(u, x);
-  uint32_t w[VW / 4];
+// four integers as bytes: t = 1.5 2^23 + (x / s rounded) has the integer in its low bits, and x - q s is exact (a multiple
+// of s's last place, and no larger than about s), so it tells whether the integer is the nearest one, or has a rival
+__device__ __forceinline__ uint32_t four_bytes(const float *x, float s, float inv) {
+  float off = 0.0f;
+  uint32_t t[4];
 #pragma unroll
-  for (int i = 0; i < VW / 4; i++) {
-    uint32_t b = 0;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      // s 0: the block holds zeros (or values under half a step of the smallest float); s NaN: it held none
-      const int q = s > 0 ? nearest(x[4 * i + j], s, inv) : 0;
-      b |= (uint32_t)(q & 255) << (8 * j);
-    }
-    w[i] = b;
+  for (int j = 0; j < 4; j++) {
+    const float z = __fmaf_rn(x[j], inv, 12582912.0f);
+    t[j] = __float_as_uint(z);
+    off = fmaxf(off, fabsf(__fmaf_rn(-(z - 12582912.0f), s, x[j])));
   }
-  if (VW == 8) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[VW / 4 - 1]);
-  else *reinterpret_cast<uint32_t *>(dst) = w[0];
+  if (off + off >= s) {
+#pragma unroll 1
+    for (int j = 0; j < 4; j++) t[j] = (uint32_t)exactly(x[j], s);
+  }
+  return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+}
+// four earlier integers from scale a to scale b, ratio about a / b (q a is rounded here: by 2^-24 of 127 b at most)
+__device__ __forceinline__ uint32_t four_moved(uint32_t q4, float a, float b, float ratio) {
+  float off = 0.0f;
+  uint32_t t[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const float q = (float)(int8_t)(q4 >> (8 * j)), z = __fmaf_rn(q, ratio, 12582912.0f);
+    t[j] = __float_as_uint(z);
+    off = fmaxf(off, fabsf(__fmaf_rn(-(z - 12582912.0f), b, __fmul_rn(q, a))));
+  }
+  if (off + off > b * 0.99997f) {
+#pragma unroll 1
+    for (int j = 0; j < 4; j++) t[j] = (uint32_t)exactly((double)(int8_t)(q4 >> (8 * j)) * a, b);
+  }
+  return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 
 struct StoreArgs {
@@ -298,30 +321,51 @@ struct StoreArgs {
   int n, blocks, block, nkv, hs, per;
 };
 
-template <bool HALF>
-__global__ void __launch_bounds__(ST) cache8_store_kernel(StoreArgs a) {
+// A team (TEAM threads: a block, or a warp of one) a head, its keys or its values, for the runs that begin among `per`
+// tokens.
+template <bool HALF, int TEAM>
+__global__ void __launch_bounds__(ST, 8) cache8_store_kernel(StoreArgs a) {
   pdl_begin();
   constexpr int VW = HALF ? 8 : 4;  // values of a 16-byte vector
-  __shared__ uint32_t top[ST / 32];
-  const int tid = threadIdx.x, h = blockIdx.y;
-  const bool second = blockIdx.z;  // keys, then values
+  __shared__ float top_s[2][ST / 32];
+  const int lane = threadIdx.x & 31, tid = threadIdx.x % TEAM;
+  const int unit = TEAM == ST ? blockIdx.y : blockIdx.y * (ST / TEAM) + threadIdx.x / TEAM;
+  if (unit >= 2 * a.nkv) return;
+  const bool second = unit >= a.nkv;
+  const int h = second ? unit - a.nkv : unit;
   int8_t *cache = second ? a.cache[1] : a.cache[0];
   float *scales = second ? a.scales[1] : a.scales[0];
-  const char *x = reinterpret_cast<const char *>(second ? a.x[1] : a.x[0]);
-  const int64_t stride = second ? a.stride[1] : a.stride[0];
-  const int vpr = a.hs / VW, rows = ST / vpr, row = tid / vpr, col = (tid % vpr) * VW;
-  const int i0 = blockIdx.x * a.per, i1 = min(a.n, i0 + a.per), lane = tid & 31;
-  // the block of token i, or -1 (every warp looks the slots over by itself, a lane a token)
+  const int64_t step = (second ? a.stride[1] : a.stride[0]) * (HALF ? 2 : 4);
+  const int i0 = blockIdx.x * a.per, i1 = min(a.n, i0 + a.per);
+  // a row by vpr threads, `rows` rows at a time (a row of more vectors than a warp has lanes: in two parts)
+  const int vectors = a.hs / VW, parts = vectors > TEAM ? 2 : 1, vpr = vectors / parts, rows = TEAM / vpr;
+  const int row = tid / vpr, col = (tid - row * vpr) * VW;
+  const char *x = reinterpret_cast<const char *>(second ? a.x[1] : a.x[0]) + (int64_t)i0 * step +
+                  ((int64_t)h * a.hs + col) * (HALF ? 2 : 4);
+  // a single token's vector, on its way before its slot is known
+  uint4 first = make_uint4(0, 0, 0, 0);
+  if (TEAM < ST && row == 0) first = __ldg(reinterpret_cast<const uint4 *>(x));
+  const uint32_t inverse = inverse_of(a.block);
+  // the block of token i, or -1 (a lane a token, every warp by itself)
   auto page_of = [&](int i) {
-    const int slot = i >= 0 && i < a.n ? a.slots[i] : -1, page = slot / a.block;
-    return slot >= 0 && page < a.blocks ? page : -1;
+    const int slot = i >= 0 && i < a.n ? __ldg(a.slots + i) : -1;
+    const int page = slot < 0 ? -1 : over(slot, a.block, inverse);
+    return page < a.blocks ? page : -1;
   };
-  const int mine = i0 + lane < i1 ? page_of(i0 + lane) : -1;
-  uint32_t begins = __ballot_sync(0xffffffffu, mine >= 0 && mine != page_of(i0 + lane - 1));
+  const int mine = page_of(i0 + lane), next = page_of(i0 + lane + 1);
+  int before = __shfl_up_sync(0xffffffffu, mine, 1);
+  if (lane == 0) before = page_of(i0 - 1);
+  uint32_t begins = __ballot_sync(0xffffffffu, i0 + lane < i1 && mine >= 0 && mine != before);
+  const uint32_t ends = __ballot_sync(0xffffffffu, mine != next);  // the last token of its block's run
+  int turn = 0;
   for (; begins; begins &= begins - 1) {
-    const int i = i0 + __ffs(begins) - 1, page = __shfl_sync(0xffffffffu, mine, i - i0), slot = a.slots[i];
-    int m = 1;  // the run of tokens of this block
-    for (;;) {
+    const int k = __ffs(begins) - 1, i = i0 + k, page = __shfl_sync(0xffffffffu, mine, k);
+    const int slot = __ldg(a.slots + i), held = slot - page * a.block;  // held: earlier tokens in the block
+    float *scale = scales + (int64_t)page * a.nkv + h;
+    const float s_old = held ? *scale : 0.0f;
+    const uint32_t end = ends >> k;
+    int m = end ? __ffs(end) : 32 - k;  // the run of tokens of this block, at least so far as these 32 go
+    while (!end) {
       const uint32_t other = __ballot_sync(0xffffffffu, page_of(i + m + lane) != page);
       if (other) {
         m += __ffs(other) - 1;
@@ -329,69 +373,71 @@ __global__ void __launch_bounds__(ST) cache8_store_kernel(StoreArgs a) {
       }
       m += 32;
     }
-    const int held = slot - page * a.block;  // earlier tokens in the block
-    int8_t *dst = cache + ((int64_t)page * a.nkv + h) * a.block * a.hs;
-    float *scale = scales + (int64_t)page * a.nkv + h;
-    const float s_old = held ? *scale : 0.0f;
-    const char *src = x + ((int64_t)i * stride + (int64_t)h * a.hs + col) * (HALF ? 2 : 4);
-    const int64_t step = stride * (HALF ? 2 : 4);
+    // this thread's vectors: of rows row, row + rows, ..., a row's parts one after the other
+    const int mine_of = row < rows ? (m * parts - row + rows - 1) / rows : 0;
+    const char *src = x + k * step;
+    auto vector = [&](int u) {
+      const int r = row + u * rows, t = parts == 2 ? r >> 1 : r;
+      return __ldg(reinterpret_cast<const uint4 *>(src + t * step + (parts == 2 ? (r & 1) * vpr * 16 : 0)));
+    };
     uint4 kept[KEEP];
-    uint32_t bits = 0;
-    if (row < rows) {
+    float top = 0.0f;
 #pragma unroll
-      for (int u = 0; u < KEEP; u++) {
-        const int t = row + u * rows;
-        if (t < m) kept[u] = *reinterpret_cast<const uint4 *>(src + t * step);
-      }
+    for (int u = 0; u < KEEP; u++)
+      if (u < mine_of) kept[u] = TEAM < ST && u == 0 && row == 0 && k == 0 ? first : vector(u);
 #pragma unroll
-      for (int u = 0; u < KEEP; u++)
-        if (row + u * rows < m) bits = max(bits, largest_bits<VW>(kept[u]));
-      for (int t = row + KEEP * rows; t < m; t += rows)
-        bits = max(bits, largest_bits<VW>(*reinterpret_cast<const uint4 *>(src + t * step)));
+    for (int u = 0; u < KEEP; u++)
+      if (u < mine_of) top = largest<VW>(top, kept[u]);
+#pragma unroll 4
+    for (int u = KEEP; u < mine_of; u++) top = largest<VW>(top, vector(u));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (TEAM == ST) {
+      // (by turns: a warp may be a run ahead of another that still reads)
+      if (lane == 0) top_s[turn][threadIdx.x >> 5] = top;
+      __syncthreads();  // (and this run's scale has been read)
+#pragma unroll
+      for (int w = 0; w < ST / 32; w++) top = max_nan(top, top_s[turn][w]);
+      turn ^= 1;
     }
-    bits = __reduce_max_sync(0xffffffffu, bits);
-    __syncthreads();  // the run before has read its maximum (and, in place, its scale)
-    if ((tid & 31) == 0) top[tid >> 5] = bits;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < ST / 32; w++) bits = max(bits, top[w]);
     // a value that is no finite number, now or among the earlier ones, makes the block's scale NaN: its values read
     // as NaN until the block is begun again
-    float s = bits < 0x7f800000u ? __fdiv_rn(__uint_as_float(bits), 127.0f) : __uint_as_float(0x7fffffffu);
+    float s = top < INFINITY ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fffffffu);
     if (!(s_old <= s)) s = s != s ? s : s_old;
     const float inv = s > 1e-37f ? __fdiv_rn(1.0f, s) : 0.0f;
+    int8_t *dst = cache + ((int64_t)page * a.nkv + h) * a.block * a.hs;
     if (tid == 0) *scale = s;
     if (s > s_old && s_old > 0) {
       // the earlier tokens' integers to the new step
-      const int words = held * a.hs / 4;
-      uint32_t *q4 = reinterpret_cast<uint32_t *>(dst);
-      for (int w = tid; w < words; w += ST) {
-        const uint32_t q = q4[w];
-        uint32_t b = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) b |= (uint32_t)(moved((int8_t)(q >> (8 * j)), s_old, s) & 255) << (8 * j);
-        q4[w] = b;
+      const float ratio = __fdiv_rn(s_old, s);
+      uint4 *q16 = reinterpret_cast<uint4 *>(dst);
+#pragma unroll 2
+      for (int w = tid; w < held * a.hs / 16; w += TEAM) {
+        const uint4 q = q16[w];
+        q16[w] = make_uint4(four_moved(q.x, s_old, s, ratio), four_moved(q.y, s_old, s, ratio),
+                            four_moved(q.z, s_old, s, ratio), four_moved(q.w, s_old, s, ratio));
       }
     }
-    if (row < rows) {
-      // a scale so small that its inverse is no float: its values over the scale brought into range first
-      const bool tiny = s > 0 && !(s > 1e-37f);
-      auto one = [&](int t, uint4 v) {
-        const int at = a.slots[i + t] - page * a.block;
-        if (tiny) {
-          float y[VW];
-          values_of(v, y);
+    // s 0: the block holds zeros (or values under half a step of the smallest float); s NaN: it held none. A scale so
+    // small that its inverse is no float: exactly() throughout (inv is 0 then, every guess 0)
+    const bool some = s > 0;
+    const int32_t *slots = a.slots + i;
+    const int base = page * a.block;
+    dst += col;
+    auto one = [&](int u, const uint4 &v) {
+      const int r = row + u * rows, t = parts == 2 ? r >> 1 : r;
+      float y[VW];
+      values_of(v, y);
+      int8_t *q = dst + (__ldg(slots + t) - base) * a.hs + (parts == 2 ? (r & 1) * vpr * VW : 0);
+      if (HALF)
+        *reinterpret_cast<uint2 *>(q) = some ? make_uint2(four_bytes(y, s, inv), four_bytes(y + VW - 4, s, inv)) : make_uint2(0, 0);
+      else *reinterpret_cast<uint32_t *>(q) = some ? four_bytes(y, s, inv) : 0;
+    };
 #pragma unroll
-          for (int j = 0; j < VW; j++) dst[at * a.hs + col + j] = (int8_t)moved(1, y[j], s);
-        } else {
-          put<VW>(dst + at * a.hs + col, v, s, inv);
-        }
-      };
-#pragma unroll
-      for (int u = 0; u < KEEP; u++)
-        if (row + u * rows < m) one(row + u * rows, kept[u]);
-      for (int t = row + KEEP * rows; t < m; t += rows) one(t, *reinterpret_cast<const uint4 *>(src + t * step));
-    }
+    for (int u = 0; u < KEEP; u++)
+      if (u < mine_of) one(u, kept[u]);
+#pragma unroll 2
+    for (int u = KEEP; u < mine_of; u++) one(u, vector(u));
   }
 }
 
@@ -425,6 +471,7 @@ __global__ void __launch_bounds__(LT) cache8_load_kernel(LoadArgs a) {
   if (v >= vpr) return;
   const int h = v * VW / a.hs, col = v * VW - h * a.hs;
   const int64_t slots_in = (int64_t)a.blocks * a.block;
+  const uint32_t inverse = inverse_of(a.block);
   const int i0 = blockIdx.x * L_TOKENS;
   int slot[L_TOKENS];
   uint2 q[L_TOKENS];
@@ -437,7 +484,7 @@ __global__ void __launch_bounds__(LT) cache8_load_kernel(LoadArgs a) {
 #pragma unroll
   for (int t = 0; t < L_TOKENS; t++) {
     if (slot[t] < 0) continue;
-    const int page = slot[t] / a.block, at = slot[t] - page * a.block;
+    const int page = over(slot[t], a.block, inverse), at = slot[t] - page * a.block;
     const int64_t ph = (int64_t)page * a.nkv + h;
     const int8_t *src = cache + (ph * a.block + at) * a.hs + col;
     if (HALF) q[t] = *reinterpret_cast<const uint2 *>(src);
@@ -447,9 +494,13 @@ __global__ void __launch_bounds__(LT) cache8_load_kernel(LoadArgs a) {
 #pragma unroll
   for (int t = 0; t < L_TOKENS; t++) {
     if (slot[t] < 0) continue;
+    // a byte less its bias is a float's low bits: 2^23 + 128 + q (converting takes the slow pipe)
     float x[VW];
 #pragma unroll
-    for (int j = 0; j < VW; j++) x[j] = __fmul_rn((float)(int8_t)((j < 4 ? q[t].x : q[t].y) >> (8 * (j & 3))), s[t]);
+    for (int j = 0; j < VW; j++) {
+      const uint32_t w = (j < 4 ? q[t].x : q[t].y) ^ 0x80808080u;
+      x[j] = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + (j & 3))) - 8388736.0f, s[t]);
+    }
     char *dst = out + ((int64_t)(i0 + t) * stride + (int64_t)v * VW) * (HALF ? 2 : 4);
     if (HALF) {
       uint32_t w[4];
@@ -513,7 +564,7 @@ extern "C" int b200k_block_tables(int32_t *tables, int32_t *ring, int32_t *state
     if (block < 16 || block > 256 || block % 16)
       return fail(B200FWD_EINVAL, "block_tables: a block is a multiple of 16 positions, at most 256");
     if (blocks < 1 || (int64_t)blocks * block > INT32_MAX || table_width < 1 ||
-        (int64_t)table_width * block > INT32_MAX)
+        (int64_t)table_width * block > INT32_MAX / 2)
       return fail(B200FWD_EINVAL, "block_tables: 1 block at least, and positions and slots that an int32 holds");
     TablesArgs a = {tables, ring, state_out, lengths_out, starts, slots, seq, pos, state, lengths, news,
                     n_seqs, table_width, blocks, block, n};
@@ -552,9 +603,17 @@ extern "C" int b200k_cache8_store(int8_t *kc, float *ks, int8_t *vc, float *vs, 
     if (!rc) rc = check_rows("cache8_store", v, v_stride, (int64_t)nkv * hs, half);
     if (rc) return rc;
     StoreArgs a = {{kc, vc}, {ks, vs}, {k, v}, {k_stride, v_stride}, slots, n, blocks, block, nkv, hs, 0};
-    a.per = n <= 256 ? 1 : n <= 2048 ? 4 : 16;
-    const dim3 grid((n + a.per - 1) / a.per, nkv, 2);
-    launch(half ? cache8_store_kernel<true> : cache8_store_kernel<false>, grid, dim3(ST), 0, as_stream(stream), a);
+    // Up to 512 tokens a warp each (and head), so that single ones are stored side by side; else a thread block for the runs
+    // that begin among 16, which are few where prompts are stored.
+    if (n <= 512) {
+      a.per = 1;
+      launch(half ? cache8_store_kernel<true, 32> : cache8_store_kernel<false, 32>, dim3(n, (2 * nkv + 3) / 4), dim3(ST), 0,
+             as_stream(stream), a);
+    } else {
+      a.per = 16;
+      launch(half ? cache8_store_kernel<true, ST> : cache8_store_kernel<false, ST>, dim3((n + 15) / 16, 2 * nkv), dim3(ST), 0,
+             as_stream(stream), a);
+    }
     B200_LAUNCHED("cache8_store");
     return 0;
   } catch (...) {

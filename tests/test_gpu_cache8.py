@@ -161,7 +161,7 @@ def store_case(k, v, slots, blocks, block, nkv, hs, half, seed, pad=0, kv=None):
     return (kc, ks), (vc, vs)
 
 
-SHAPES = [(1, 16, 16), (2, 48, 16), (8, 128, 32), (3, 64, 64), (2, 80, 48), (1, 256, 256), (5, 96, 16), (4, 112, 128)]
+SHAPES = [(1, 16, 16), (2, 48, 16), (1, 144, 32), (8, 128, 32), (3, 64, 64), (2, 80, 48), (1, 256, 256), (5, 96, 16), (4, 112, 128)]
 
 
 @pytest.mark.parametrize("half", [False, True])
