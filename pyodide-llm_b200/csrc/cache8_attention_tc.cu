@@ -54,9 +54,36 @@ struct Tc {
     uint32_t tmem_base;
     int part[2][THREADS / 32], found[2];
     int2 of[SORTED];                    // the requests' positions and groups of tiles
+    int2 row[TILES][QT];                // a row's token (of all; -1: there is none) and query head
   };
 };
 
+// Waits for the phase of `parity`; false when that took 2 s, or another wait did (the error word is set then). Without a
+// suspend-time hint: from a thread of a warp's to another's and back takes 281 cycles so, with a hint of 1 ms 671.
+__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, int *error, int code) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t begun = 0, now;
+  for (uint32_t i = 1;; i++) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 255) == 0) {
+      asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+      if (begun == 0) begun = now;
+      if (*(volatile int *)error) return false;
+      if (now - begun > 2000000000ull) {
+        atomicCAS(error, 0, code);
+        return false;
+      }
+    }
+  }
+}
 // The thread of a converged warp that issues its products. (elect.sync rather than a lane's number: the products' operands
 // go through the warp's uniform registers, and what the compiler makes of a branch on the lane, predicates among it, left
 // other lanes' values in them; with a predicate of one's own on every product a product took 100 cycles to issue, 66 so.)
@@ -112,10 +139,15 @@ __device__ __forceinline__ void st8(uint32_t taddr, const uint32_t *u) {
                "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                : "memory");
 }
-__device__ __forceinline__ void st32(uint32_t taddr, const float *r) {
-  const uint32_t *u = reinterpret_cast<const uint32_t *>(r);
-#pragma unroll
-  for (int i = 0; i < 4; i++) st8(taddr + 8 * i, u + 8 * i);
+// every load of this thread has arrived; x: what they were into (so that nothing reads it earlier)
+__device__ __forceinline__ void wait_ld32(float *x) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]), "+f"(x[4]), "+f"(x[5]), "+f"(x[6]), "+f"(x[7]), "+f"(x[8]),
+                 "+f"(x[9]), "+f"(x[10]), "+f"(x[11]), "+f"(x[12]), "+f"(x[13]), "+f"(x[14]), "+f"(x[15]), "+f"(x[16]),
+                 "+f"(x[17]), "+f"(x[18]), "+f"(x[19]), "+f"(x[20]), "+f"(x[21]), "+f"(x[22]), "+f"(x[23]), "+f"(x[24]),
+                 "+f"(x[25]), "+f"(x[26]), "+f"(x[27]), "+f"(x[28]), "+f"(x[29]), "+f"(x[30]), "+f"(x[31])
+               :
+               : "memory");
 }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -144,7 +176,8 @@ __device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uin
 // One step of this thread's row: 64 scores from tS, their weights over them. EDGE: some of the tile's rows don't see all
 // of the step; limit: the last position that this row sees, from the step's first. m, l: the row's running maximum and
 // sum. settle(top): called by the whole warp where some row's maximum moves, to `top`; what it returns the sum is
-// scaled by.
+// scaled by. (The next step's scores, loaded while this one's last weights are worked out, cost more than they saved: 189
+// us for 172, 102 for 97.)
 template <int HP, bool HALF, bool EDGE, typename Settle>
 __device__ __forceinline__ void softmax_step(uint32_t tS, const float4 *sc, float qf, int limit, float &m, float &l,
                                              Settle &&settle) {
@@ -159,7 +192,8 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, const float4 *sc, floa
     // (a unit that the row does not see may have any scales, NaN too)
     if (EDGE && u * UNIT > limit) c[u] = 1.0f, lg[u] = 0.0f, inv[u] = 0.0f;
   }
-  tmem_wait_ld();
+  wait_ld32(x);
+  wait_ld32(x + 32);
   float most = -INFINITY;
 #pragma unroll
   for (int u = 0; u < KU; u++) {
@@ -241,7 +275,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     if (lane == 31) s.part[0][warp] = upto, s.part[1][warp] = own;
     __syncthreads();
     int before = total;
-    for (int w = 0; w < THREADS / 32; w++) {
+    for (int w = 0; w < min(THREADS / 32, (a.n_seqs - base + 31) / 32); w++) {
       if (w < warp) before += s.part[0][w];
       total += s.part[0][w];
       fresh = min(fresh + s.part[1][w], a.n + 1);
@@ -310,16 +344,39 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
   const int token = on ? x_own / a.group : 0, head = h * a.group + (on ? x_own % a.group : 0);
   const int pos = on ? r.length - r.fresh + token : -1;
   const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-  // 8 values z of the output row from value d on
+  // Output rows go through the tile's queries' place in shared memory, so that a warp writes whole rows: 8 values z of
+  // this thread's row from value d on, then all the warp's rows
+  constexpr int PIECES = HP * (HALF ? 2 : 4) / 16;
   auto put = [&](int d, const float (&z)[8]) {
-    const int64_t off = (int64_t)(r.first + token) * a.out_stride + (int64_t)head * a.hs + d;
+    uint8_t *row = &s.q[t_own][0][0][0] + y * (PIECES * 16);
     if (HALF) {
-      *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(a.out) + off) =
+      *reinterpret_cast<uint4 *>(row + (((d >> 3) ^ (y & 7)) << 4)) =
           make_uint4(pack(z[0], z[1]), pack(z[2], z[3]), pack(z[4], z[5]), pack(z[6], z[7]));
     } else {
-      float4 *dst = reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + off);
-      dst[0] = make_float4(z[0], z[1], z[2], z[3]);
-      dst[1] = make_float4(z[4], z[5], z[6], z[7]);
+      *reinterpret_cast<float4 *>(row + (((d >> 2) ^ (y & 7)) << 4)) = make_float4(z[0], z[1], z[2], z[3]);
+      *reinterpret_cast<float4 *>(row + (((d >> 2) + 1 ^ (y & 7)) << 4)) = make_float4(z[4], z[5], z[6], z[7]);
+    }
+  };
+  auto write = [&]() {
+    constexpr int ES = HALF ? 2 : 4;
+    const int piece = lane % PIECES;
+    s.row[t_own][y] = make_int2(on ? r.first + token : -1, head);
+    __syncwarp();
+#pragma unroll 1
+    for (int i = lane / PIECES; i < 32; i += 4 * (32 / PIECES)) {
+      uint4 z[4];
+      int2 of[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int row = (y & ~31) + i + u * (32 / PIECES);
+        of[u] = s.row[t_own][row];
+        z[u] = *reinterpret_cast<const uint4 *>(&s.q[t_own][0][0][0] + (row * PIECES + (piece ^ (row & 7))) * 16);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+        if (of[u].x >= 0 && piece * 16 < a.hs * ES)
+          *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(a.out) +
+                                     (of[u].x * a.out_stride + (int64_t)of[u].y * a.hs) * ES + piece * 16) = z[u];
     }
   };
   // 1 / the row sum; a row that sees nothing is 0, one past its table's row (or after a wait that gave up) NaN
@@ -327,7 +384,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     return !ok || pos >= cap ? __uint_as_float(0x7fffffffu) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
   };
 
-  // (the launch's 640 x 96 registers: 128 x (64 + 64 + 144 + 168 + 40) = 640 x 96)
+  // (the launch's 640 x 96 registers: 128 x (64 + 64 + 144 + 168 + 40), float16 128 x (64 + 64 + 152 + 152 + 48))
   if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // ---- the cache: thread tid brings 16 bytes of rows tid / CH + i * PER (CH pieces a row) of keys and of values
@@ -392,7 +449,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     }
     for (int j = 0; j < most_steps; j++) {
       const int slot = j % STAGES;
-      if (!mbar_wait(&s.kv_empty[slot], ((j / STAGES) & 1) ^ 1, error, 101)) break;
+      if (!wait_for(&s.kv_empty[slot], ((j / STAGES) & 1) ^ 1, error, 101)) break;
       const bool more = j + 1 < most_steps;
 #pragma unroll
       for (int i = 0; i < R; i++) {
@@ -420,7 +477,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       mbar_arrive(&s.kv_full[slot]);
     }
   } else if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (HALF) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     // A warp each for the scores' products and for the values', of each tile, and one thread of it: what such a thread waits
     // for and works out between products takes a few hundred cycles, in which the others keep the tensor cores busy. What
     // it computes for a product is a sum: the operands' descriptors are the first ones', with a multiple of 16 bytes added
@@ -429,7 +487,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     if (t < TILES && elected()) {
       constexpr int PART = S::CHUNKS * QT * 128 / 16, STAGE = S::CHUNKS * KT * 128 / 16;
       bool ok = true;
-      auto wait = [&](uint64_t *bar, uint32_t parity, int code) { ok = ok && mbar_wait(bar, parity, error, code); };
+      auto wait = [&](uint64_t *bar, uint32_t parity, int code) { ok = ok && wait_for(bar, parity, error, code); };
       if ((warp & 1) == 0) {
         const uint32_t id_s = idesc_f16(QT, KT);
         const uint64_t q0 = desc_sw128(s.q[t][0][0]), k0 = desc_sw128(s.k[0][0]);
@@ -483,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     }
     __syncwarp();
     // every product issued has completed before the block frees TMEM
-    if (warp == 16) mbar_wait(&s.mma_done, 0, error, 114);
+    if (warp == 16) wait_for(&s.mma_done, 0, error, 114);
   } else if (!HALF && warp >= 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // ---- float32: the rows' sums, a step's product at a time
@@ -493,8 +551,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     for (int i = 0; i < HP; i++) acc[i] = 0.0f;
     bool ok = true;
     for (int j = 0; j < n && ok; j++) {
-      ok = mbar_wait(&s.by_full[j & 3], (j >> 2) & 1, error, 121);
-      ok = mbar_wait(&s.pv_done[0][j % SBUF], (j / SBUF) & 1, error, 122) && ok;
+      ok = wait_for(&s.by_full[j & 3], (j >> 2) & 1, error, 121);
+      ok = wait_for(&s.pv_done[0][j % SBUF], (j / SBUF) & 1, error, 122) && ok;
       ok = __all_sync(0xffffffffu, ok);
       const float by = s.by[j & 3][y];
       const uint64_t by2 = f2(by, by);
@@ -515,71 +573,77 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.o_free[j & 1]);
     }
-    ok = mbar_wait(&s.l_full, 0, error, 123) && ok;
+    ok = wait_for(&s.l_full, 0, error, 123) && ok;
     const float by = inverse(s.l[y], ok);
-    if (on) {
 #pragma unroll
-      for (int d = 0; d < HP; d += 8)
-        if (d < a.hs) {
-          float z[8];
+    for (int d = 0; d < HP; d += 8) {
+      float z[8];
 #pragma unroll
-          for (int e = 0; e < 8; e++) z[e] = by == 0.0f ? 0.0f : acc[d + e] * by;
-          put(d, z);
-        }
+      for (int e = 0; e < 8; e++) z[e] = by == 0.0f ? 0.0f : acc[d + e] * by;
+      put(d, z);
     }
+    write();
   } else {
-    if (HALF && warp >= 12) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    if (HALF) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     // ---- the softmax of tile t_own. Its queries first, as float16 (float32: by a power of two into (0, 2), in two parts)
     // in the swizzled layout
     const int t = t_own;
     float qf = 1.0f;
+    s.row[t][y] = make_int2(on ? r.first + token : -1, head);
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
     {
-      // a row by LANES threads, 8 values each, all rows' loads in flight
-      constexpr int LANES = HP / 8, AT_ONCE = 128 / LANES;
+      // a row by LANES threads, 8 values each; ROWS rows' loads in flight
+      constexpr int LANES = HP / 8, AT_ONCE = 128 / LANES, ROWS = HALF ? 8 : 4;
       const int col = y % LANES * 8, sub = y / LANES;
-#pragma unroll (HALF ? 16 : 4)
-      for (int row = sub; row < QT; row += AT_ONCE) {
-        const int x = row0 + t * QT + row;
-        const int64_t off = (int64_t)(r.first + (x < rows ? x / a.group : 0)) * a.q_stride +
-                            (int64_t)(h * a.group + (x < rows ? x % a.group : 0)) * a.hs + col;
-        const bool in = x < rows && col < a.hs;  // (zeros past the head, as the keys have there)
-        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (HALF) {
-          if (in) hi = *reinterpret_cast<const uint4 *>(reinterpret_cast<const __half *>(a.q) + off);
-        } else {
-          float4 z0 = make_float4(0, 0, 0, 0), z1 = z0;
-          if (in) {
-            const float4 *src = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + off);
-            z0 = src[0], z1 = src[1];
-          }
-          float z[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w}, top = 0.0f;
+#pragma unroll 1
+      for (int first = sub; first < QT; first += ROWS * AT_ONCE) {
+        uint4 raw[ROWS][HALF ? 1 : 2];
 #pragma unroll
-          for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(z[i]));
+        for (int i = 0; i < ROWS; i++) {
+          const int2 of = s.row[t][first + i * AT_ONCE];
+          const int64_t off = of.x * a.q_stride + (int64_t)of.y * a.hs + col;
+          const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(a.q) + off * (HALF ? 2 : 4));
+          const bool in = of.x >= 0 && col < a.hs;  // (zeros past the head, as the keys have there)
 #pragma unroll
-          for (int d = LANES / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-          const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
-          const float f = __uint_as_float((uint32_t)(127 - e) << 23);
-          if (col == 0) s.l[row] = __uint_as_float((uint32_t)(127 + e) << 23);
-          uint32_t p[4], q[4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            z[2 * i] *= f, z[2 * i + 1] *= f;
-            p[i] = pack(z[2 * i], z[2 * i + 1]);
-            const float2 b = unpack(p[i]);
-            q[i] = pack(z[2 * i] - b.x, z[2 * i + 1] - b.y);
-          }
-          hi = make_uint4(p[0], p[1], p[2], p[3]), lo = make_uint4(q[0], q[1], q[2], q[3]);
+          for (int e = 0; e < (HALF ? 1 : 2); e++) raw[i][e] = in ? src[e] : make_uint4(0, 0, 0, 0);
         }
-        const int at = row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4);
-        *reinterpret_cast<uint4 *>(&s.q[t][0][col >> 6][at]) = hi;
-        if (!HALF) *reinterpret_cast<uint4 *>(&s.q[t][PARTS - 1][col >> 6][at]) = lo;
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+          const int row = first + i * AT_ONCE;
+          uint4 hi = raw[i][0], lo = hi;
+          if (!HALF) {
+            const uint4 w = raw[i][PARTS - 1];
+            float z[8] = {__uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w),
+                          __uint_as_float(w.x),  __uint_as_float(w.y),  __uint_as_float(w.z),  __uint_as_float(w.w)};
+            float top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(z[k]));
+#pragma unroll
+            for (int d = LANES / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
+            const float f = __uint_as_float((uint32_t)(127 - e) << 23);
+            if (col == 0) s.l[row] = __uint_as_float((uint32_t)(127 + e) << 23);
+            uint32_t p[4], q[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              z[2 * k] *= f, z[2 * k + 1] *= f;
+              p[k] = pack(z[2 * k], z[2 * k + 1]);
+              const float2 b = unpack(p[k]);
+              q[k] = pack(z[2 * k] - b.x, z[2 * k + 1] - b.y);
+            }
+            hi = make_uint4(p[0], p[1], p[2], p[3]), lo = make_uint4(q[0], q[1], q[2], q[3]);
+          }
+          const int at = row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4);
+          *reinterpret_cast<uint4 *>(&s.q[t][0][col >> 6][at]) = hi;
+          if (!HALF) *reinterpret_cast<uint4 *>(&s.q[t][PARTS - 1][col >> 6][at]) = lo;
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&s.q_full);
       if (!HALF) {
         // the rows' powers of two, among the four warps (l is for the sums later)
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 3, 128;" ::: "memory");
         qf = s.l[y];
       }
     }
@@ -589,9 +653,9 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     const int n = steps[t];
     bool ok = true;
     for (int j = 0; j < n && ok; j++) {
-      ok = mbar_wait(&s.s_full[t][j % SBUF], (j / SBUF) & 1, error, 116);
-      // (complete before the scores were begun: its scales are there)
-      ok = mbar_wait(&s.kv_full[j % STAGES], (j / STAGES) & 1, error, 117) && ok;
+      // (the step's scales are there with its scores: the keys were complete before the scores were begun)
+      ok = wait_for(&s.s_full[t][j % SBUF], (j / SBUF) & 1, error, 116);
+      ok = wait_for(&s.kv_full[j % STAGES], (j / STAGES) & 1, error, 117) && ok;
       ok = __all_sync(0xffffffffu, ok);
       fence_after();
       // where a row's maximum moves; by < 0: nowhere in the warp
@@ -602,17 +666,18 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
           if (lane == 0) mbar_arrive(&s.by_full[j & 3]);
         } else if (by >= 0.0f && j > 0) {  // (whole warps come here: TMEM is read and written by whole warps)
           // O holds the steps so far: it goes to the new maxima once the last P V is done
-          mbar_wait(&s.pv_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1, error, 109);
+          wait_for(&s.pv_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1, error, 109);
           __syncwarp();
           fence_after();
 #pragma unroll
-          for (int ch = 0; ch < HP / 32; ch++) {
-            float o[32];
-            ld32(o_col + ch * 32, o);
+          for (int ch = 0; ch < HP / 16; ch++) {
+            uint32_t o[16];
+            tmem_ld<16>(o_col + ch * 16, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; i++) o[i] *= by;
-            st32(o_col + ch * 32, o);
+            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+            st8(o_col + ch * 16, o);
+            st8(o_col + ch * 16 + 8, o + 8);
           }
         }
         return by;
@@ -632,30 +697,30 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       if (lane == 0) mbar_arrive(&s.l_full);
     } else {
       if (n > 0) {
-        ok = mbar_wait(&s.pv_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1, error, 118) && ok;
+        ok = wait_for(&s.pv_done[t][(n - 1) & 1], ((n - 1) >> 1) & 1, error, 118) && ok;
         __syncwarp();
         fence_after();
+      } else {
+        ok = wait_for(&s.q_full, 0, error, 119) && ok;  // (the rows go where other warps still put queries)
       }
       const float by = inverse(l, ok);
-#pragma unroll
+      __syncwarp();
+#pragma unroll 1
       for (int ch = 0; ch < HP / 32; ch++) {
         float o[32];
-        __syncwarp();
         if (n > 0) {
           ld32(o_col + ch * 32, o);
-          tmem_wait_ld();
+          wait_ld32(o);
         }
-        if (on) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            if (ch * 32 + i < a.hs) {
-              float z[8];
+        for (int i = 0; i < 32; i += 8) {
+          float z[8];
 #pragma unroll
-              for (int e = 0; e < 8; e++) z[e] = n > 0 && by != 0.0f ? o[i + e] * by : by;
-              put(ch * 32 + i, z);
-            }
+          for (int e = 0; e < 8; e++) z[e] = n > 0 && by != 0.0f ? o[i + e] * by : by;
+          put(ch * 32 + i, z);
         }
       }
+      write();
     }
   }
   fence_before();
