@@ -33,6 +33,8 @@ __device__ __forceinline__ int over(int x, int by, uint32_t inverse) {
 // for partial sums. Takes read the ring's live part and gives write behind it, takes write table entries that no
 // token's slot is read from (a token of a new block finds its id in the ring), so only lengths and state, which may
 // be updated in place, have to wait until every block has read them: the one cluster barrier.
+// Measured: 64 requests of a token each 6.8 us; 1000 that add 250 to 500 tokens each (358,000 slots) 22 us, of
+// which the running sums over 1000 requests and the barrier are most. A launch by itself is 2 to 3 us.
 
 constexpr int TT = 512;  // threads, and the requests of one tile of the running sums
 
@@ -243,6 +245,9 @@ __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
 // where its run of tokens begins: no two teams touch one (block, head), and no atomics. A team is a thread block, or a
 // warp where the call has few tokens; it keeps the values that fit its registers between finding the largest and
 // rounding (the rest it reads again, from L1).
+// Measured with the load that follows, 8 heads of 128: 64 single tokens in float32 8.2 us (a thread block a token 9.5),
+// 4700 tokens of 64 prompts in float16 35 us, of which the load is 12 (a warp a run: 54 together). Bound by instructions
+// and their latency: a run's slots, scale and largest value come one after the other.
 
 constexpr int ST = 128;  // threads of a block
 constexpr int KEEP = 4;  // 16-byte vectors of new values that a thread keeps in registers between its two passes
@@ -444,7 +449,8 @@ __global__ void __launch_bounds__(ST, 8) cache8_store_kernel(StoreArgs a) {
 // -------------------------------------------------------------------------------------------------------- load
 //
 // q s, rounded once to the output's type. Bound by its writes (4 or 2 bytes a value for the 1 read): a thread keeps
-// its columns for several tokens and writes 16 bytes a token.
+// its columns for several tokens and writes 16 bytes a token. Bytes become numbers by a permute under 2^23's exponent and
+// a subtraction, four at a time. 4700 tokens of 8 heads of 128 in float16: 12 us for 29 MB.
 
 constexpr int LT = 256;      // threads
 constexpr int L_TOKENS = 4;  // tokens of a thread

@@ -16,8 +16,12 @@
 //     cut off rather than rounded: over 2048 positions that came to 2.5e-6 of the outputs, of one step it is nothing.)
 //   warps 16..19 issue the products, two a tile: S = Q K^T (M 128, N 64; float32: once for each part of Q) and O = P V
 //     (M 128, N head size; float32: once for each part of P) with P read from TMEM.
-// Bound by the tensor cores and, close behind, by instructions issued (float16, heads of 128: a step is 1024 cycles of
-// products, as many of exponentials, and about as many issue slots, a third of them for widening).
+// What bounds it, in cycles. Float16, heads of 128: a step of both tiles takes 2330, of which the products are 1540 (S with
+// its N of 64 at half rate: 63 for each 16 of K, as Q comes from shared memory every time; P V 66), exponentials 1024,
+// issue slots 1400; a block begins and ends in 15,000 (the queries, the first keys, the first scores; rows out) beside 30
+// steps on average. Float32, heads of 64: 2060 a step, one after the other a row's scores, weights and their two parts.
+// Measured: 8 requests that add 260 to 509 tokens to contexts of up to 4500, 32 query and 8 kv heads of 128, float16: 172 us
+// (0.64 PFLOP/s of what the masks leave); 4 whole prompts of 2048 tokens, 8 heads of 64, float32: 97 us.
 // TMEM (512 columns), float16: tile t's two score buffers at 128 t + {0, 64}, its O at 256 + t * head size; float32: three
 // score buffers at {0, 64, 128}, two of O at 192 + {0, 1} * head size.
 // Every wait is bounded: past it the kernel sets the scratch's error word and runs to its end.
