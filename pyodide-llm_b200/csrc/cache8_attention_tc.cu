@@ -383,9 +383,10 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
                                      (of[u].x * a.out_stride + (int64_t)of[u].y * a.hs) * ES + piece * 16) = z[u];
     }
   };
-  // 1 / the row sum; a row that sees nothing is 0, one past its table's row (or after a wait that gave up) NaN
+  // 1 / the row sum; a row that sees nothing is 0, one past its table's row, without any weight (all its scores -inf, of an
+  // infinite query) or after a wait that gave up NaN
   auto inverse = [&](float l, bool ok) {
-    return !ok || pos >= cap ? __uint_as_float(0x7fffffffu) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    return pos < 0 && ok ? 0.0f : !ok || pos >= cap || l == 0.0f ? __uint_as_float(0x7fffffffu) : __fdiv_rn(1.0f, l);
   };
 
   // (the launch's 640 x 96 registers: 128 x (64 + 64 + 144 + 168 + 40), float16 128 x (64 + 64 + 152 + 152 + 48))

@@ -474,6 +474,26 @@ def test_attention_of_queries_of_any_size(size):
     c.check(c.run())
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("hs", [48, 128])
+def test_attention_of_queries_that_are_no_numbers(hs, half):
+    """A query with an infinity or a NaN in it gives NaN, and changes no other row or head. (The keys of the first block
+    are such that an infinity's scores are all -inf there.)"""
+    c = Case([(50, 1), (60, 20), (150, 100), (100, 100)], 4, 2, hs, 16, half, seed=11)
+    c.kc[c.tables[3, 0], :, :, 1] = -np.abs(c.kc[c.tables[3, 0], :, :, 1]) - 1
+    want = c.run()
+    c.check(want)
+    odd = [(0, 1, np.nan), (5, 0, np.inf), (20, 3, -np.inf), (21, 2, np.nan), (77, 1, np.inf), (120, 3, -np.inf),
+           (121, 0, np.inf), (125, 2, np.inf), (200, 3, np.nan)]
+    is_odd = np.zeros((c.n, c.heads), bool)
+    for row, head, x in odd:
+        c.q[row, head * hs + 1] = x
+        is_odd[row, head] = True
+    got = c.run()
+    assert np.isnan(got[is_odd]).all(), np.argwhere(~np.isnan(got).any(2) & is_odd)
+    assert np.array_equal(got[~is_odd], want[~is_odd])
+
+
 def test_attention_sharp_and_growing_scores():
     """The running maximum moves at every unit, up to scores in the hundreds."""
     c = Case([(400, 1), (300, 30)], 4, 2, 64, 16, False, seed=10)
