@@ -37,7 +37,6 @@ namespace {
 using namespace tc;
 
 constexpr int QT = 128, KT = 64, THREADS = 640, KU = KT / UNIT;
-constexpr int BRINGERS = 256;  // threads that bring the cache
 constexpr int SORTED = 64;     // requests that are taken in order of their lengths
 
 template <int HP, bool HALF>
@@ -46,15 +45,19 @@ struct Tc {
   static constexpr int CHUNKS = HP / 64;  // 128-byte columns of 64 float16
   static constexpr int PARTS = HALF ? 1 : 2;
   static constexpr int STAGES = 4;
-  static constexpr int SBUF = HALF ? 2 : 3;  // score buffers of a tile
+  // float32, heads of up to 64: two warpgroups of softmax (of even and odd steps), and four warps that bring the cache
+  static constexpr int SOFT = !HALF && HP == 64 ? 2 : 1, BRINGERS = SOFT == 2 ? 128 : 256;
+  static constexpr int SBUF = HALF ? 2 : 2 + SOFT;  // score buffers of a tile
   struct Smem {
     alignas(1024) uint8_t q[TILES][PARTS][CHUNKS][QT * 128];
     alignas(1024) uint8_t k[STAGES][CHUNKS][KT * 128];
     alignas(1024) uint8_t v[STAGES][CHUNKS][KT * 128];
     alignas(16) float4 sc[STAGES][KU];  // a unit's {key scale * log2(e) / sqrt(hs), log2(value scale), 1 / value scale}
-    float by[4][QT], l[QT];             // float32: what the rows' sums so far are scaled by at a step; the row sums
+    // float32: the maxima that a step's weights are relative to (softmax is up to SBUF + 1 steps ahead of the sums); at the
+    // end each warpgroup's sums and maxima; the powers of two that the queries were divided by
+    float ref[8][QT], l[SOFT][QT], m[SOFT][QT], power[QT];
     uint64_t q_full, kv_full[STAGES], kv_empty[STAGES];
-    uint64_t s_full[TILES][SBUF], p_full[TILES][SBUF], pv_done[TILES][SBUF], o_free[2], by_full[4], l_full, mma_done;
+    uint64_t s_full[TILES][SBUF], p_full[TILES][SBUF], pv_done[TILES][SBUF], o_free[2], ref_full[8], l_full, mma_done;
     uint32_t tmem_base;
     int part[2][THREADS / 32], found[2];
     int2 of[SORTED];                    // the requests' positions and groups of tiles
@@ -159,6 +162,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float reciprocal(float x) {  // within 1 of the last place
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint64_t f2(float lo, float hi) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -167,6 +175,11 @@ __device__ __forceinline__ uint64_t f2(float lo, float hi) {
 __device__ __forceinline__ uint64_t fma_2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 __device__ __forceinline__ uint64_t add_2(uint64_t a, uint64_t b) {
@@ -179,8 +192,8 @@ __device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uin
 
 // One step of this thread's row: 64 scores from tS, their weights over them. EDGE: some of the tile's rows don't see all
 // of the step; limit: the last position that this row sees, from the step's first. m, l: the row's running maximum and
-// sum. settle(top): called by the whole warp where some row's maximum moves, to `top`; what it returns the sum is
-// scaled by. (The next step's scores, loaded while this one's last weights are worked out, cost more than they saved: 189
+// sum. settle(by): called by the whole warp once m is settled, where some row's maximum moved with what the
+// row's sums go down by. (The next step's scores, loaded while this one's last weights are worked out, cost more than they saved: 189
 // us for 172, 102 for 97.)
 template <int HP, bool HALF, bool EDGE, typename Settle>
 __device__ __forceinline__ void softmax_step(uint32_t tS, const float4 *sc, float qf, int limit, float &m, float &l,
@@ -213,9 +226,9 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, const float4 *sc, floa
     most = fmaxf(most, __fmaf_rn(top, c[u], lg[u]));
   }
   if (__any_sync(0xffffffffu, most > m + RESCALE)) {
-    const float top = fmaxf(m, most);
-    l *= settle(m == top ? 1.0f : ex2(m - top));
-    m = top;
+    const float top = fmaxf(m, most), by = m == top ? 1.0f : ex2(m - top);
+    l *= by, m = top;
+    settle(by);
   } else {
     settle(-1.0f);
   }
@@ -246,7 +259,7 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, const float4 *sc, floa
 template <int HP, bool HALF>
 __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const Args a) {
   using S = Tc<HP, HALF>;
-  constexpr int STAGES = S::STAGES, PARTS = S::PARTS, TILES = S::TILES, SBUF = S::SBUF;
+  constexpr int STAGES = S::STAGES, PARTS = S::PARTS, TILES = S::TILES, SBUF = S::SBUF, SOFT = S::SOFT, BRINGERS = S::BRINGERS;
   extern __shared__ uint8_t raw[];
   typename S::Smem &s = *reinterpret_cast<typename S::Smem *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   pdl_begin();
@@ -313,7 +326,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
   }
 
   if (tid == 0) {
-    mbar_init(&s.q_full, TILES * QT);
+    mbar_init(&s.q_full, TILES * SOFT * QT);
     for (int i = 0; i < STAGES; i++) {
       mbar_init(&s.kv_full[i], BRINGERS);
       mbar_init(&s.kv_empty[i], TILES);
@@ -326,8 +339,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       }
     }
     for (int u = 0; u < 2; u++) mbar_init(&s.o_free[u], 4);
-    for (int u = 0; u < 4; u++) mbar_init(&s.by_full[u], 4);
-    mbar_init(&s.l_full, 4);
+    for (int u = 0; u < 8; u++) mbar_init(&s.ref_full[u], 4);
+    mbar_init(&s.l_full, 4 * SOFT);
     mbar_init(&s.mma_done, 2 * TILES);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -389,13 +402,15 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     return pos < 0 && ok ? 0.0f : !ok || pos >= cap || l == 0.0f ? __uint_as_float(0x7fffffffu) : __fdiv_rn(1.0f, l);
   };
 
-  // (the launch's 640 x 96 registers: 128 x (64 + 64 + 144 + 168 + 40), float16 128 x (64 + 64 + 152 + 152 + 48))
-  if (warp < 8) {
+  // (the launch's 640 x 96 registers: 128 x (64 + 64 + 144 + 168 + 40), SOFT 2 128 x (64 + 128 + 128 + 120 + 40), float16
+  // 128 x (64 + 64 + 152 + 152 + 48))
+  if (warp < BRINGERS / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    // ---- the cache: thread tid brings 16 bytes of rows tid / CH + i * PER (CH pieces a row) of keys and of values
+    // ---- the cache: a thread brings 16 bytes of rows brow + i * PER (CH pieces a row) of keys and of values. Eight threads
+    // in a row take four pieces of two rows, which go to eight different 16-byte columns of the swizzled lines.
     constexpr int CH = HP / 16, PER = BRINGERS / CH, R = KT / PER;
     const int32_t *table = a.tables + (int64_t)req * a.width;
-    const int piece = tid % CH, brow = tid / CH;
+    const int piece = (tid & 3) + (tid >> 3) % (CH / 4) * 4, brow = (tid >> 2 & 1) + (tid >> 3) / (CH / 4) * 2;
     const bool in_head = piece * 16 < a.hs;
     // table entries from held on are no row's to see (or NaN rows')
     const int held = min(a.width, (r.length + a.block - 1) / a.block);
@@ -411,9 +426,12 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       if (p.at >= a.block) p.at -= a.block, p.block++;
     };
     auto page_of = [&](const Place &p) { return p.block < held ? table[p.block] : -1; };
-    auto load = [&](const int8_t *cache, int page, int at) {
-      if ((uint32_t)page >= (uint32_t)a.blocks || !in_head) return make_uint4(0, 0, 0, 0);
-      return __ldg(reinterpret_cast<const uint4 *>(cache + (int64_t)page * page_bytes + head_bytes + at * a.hs));
+    // (what is no block's, or past the head, stays any integers: the scales are NaN there, the queries 0)
+    auto load = [&](uint4 &k, uint4 &v, int page, int at) {
+      if ((uint32_t)page < (uint32_t)a.blocks && in_head) {
+        const int64_t off = (int64_t)page * page_bytes + (head_bytes + at * a.hs);
+        k = __ldg(reinterpret_cast<const uint4 *>(a.kc + off)), v = __ldg(reinterpret_cast<const uint4 *>(a.vc + off));
+      }
     };
     auto widened = [&](uint8_t *tile, int i, const uint4 &v) {
       const int row = brow + i * PER;
@@ -430,9 +448,10 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     uint4 k[R], v[R];
 #pragma unroll
     for (int i = 0; i < R; i++) {
+      k[i] = v[i] = make_uint4(0, 0, 0, 0);
       far[i] = place_of(brow + i * PER);
       const int page = most_steps > 0 ? page_of(far[i]) : -1;
-      k[i] = load(a.kc, page, far[i].at), v[i] = load(a.vc, page, far[i].at);
+      load(k[i], v[i], page, far[i].at);
       forward(far[i]);
       next[i] = most_steps > 1 ? page_of(far[i]) : -1, next_at[i] = far[i].at;
       forward(far[i]);
@@ -459,19 +478,15 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
 #pragma unroll
       for (int i = 0; i < R; i++) {
         widened(s.k[slot][0], i, k[i]);
-        if (more) k[i] = load(a.kc, next[i], next_at[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < R; i++) {
         widened(s.v[slot][0], i, v[i]);
-        if (more) v[i] = load(a.vc, next[i], next_at[i]);
+        if (more) load(k[i], v[i], next[i], next_at[i]);
         next[i] = page_of(far[i]), next_at[i] = far[i].at;
         forward(far[i]);
       }
       if (tid < KU) {
         // a key scale of 0 (a block of zeros) as the least: 0 times a masked -inf is no number
         const float c = !(ks * a.scale < 1e-30f) ? ks * a.scale : 1e-30f, w = !(vs < LEAST) ? vs : LEAST;
-        s.sc[slot][tid] = make_float4(c, __log2f(w), __fdiv_rn(1.0f, w), 0.0f);
+        s.sc[slot][tid] = make_float4(c, __log2f(w), reciprocal(w), 0.0f);
         if (more) {
           scales(spage);
           spage = page_of(sfar);
@@ -548,19 +563,24 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     // every product issued has completed before the block frees TMEM
     if (warp == 16) wait_for(&s.mma_done, 0, error, 114);
   } else if (!HALF && warp >= 12) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    if (SOFT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // ---- float32: the rows' sums, a step's product at a time
     const int n = steps[0];
     float acc[HP];
 #pragma unroll
     for (int i = 0; i < HP; i++) acc[i] = 0.0f;
+    float top = -INFINITY;
     bool ok = true;
     for (int j = 0; j < n && ok; j++) {
-      ok = wait_for(&s.by_full[j & 3], (j >> 2) & 1, error, 121);
+      ok = wait_for(&s.ref_full[j & 7], (j >> 3) & 1, error, 121);
       ok = wait_for(&s.pv_done[0][j % SBUF], (j / SBUF) & 1, error, 122) && ok;
       ok = __all_sync(0xffffffffu, ok);
-      const float by = s.by[j & 3][y];
-      const uint64_t by2 = f2(by, by);
+      // both to the larger maximum
+      const float ref = s.ref[j & 7][y], to = fmaxf(top, ref);
+      const float old_by = top == to ? 1.0f : ex2(top - to), new_by = ref == to ? 1.0f : ex2(ref - to);
+      const uint64_t old2 = f2(old_by, old_by), new2 = f2(new_by, new_by);
+      top = to;
       fence_after();
 #pragma unroll
       for (int ch = 0; ch < HP / 16; ch++) {
@@ -569,8 +589,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const uint64_t z = fma_2(f2(acc[ch * 16 + i], acc[ch * 16 + i + 1]), by2,
-                                   f2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])));
+          const uint64_t z = fma_2(f2(acc[ch * 16 + i], acc[ch * 16 + i + 1]), old2,
+                                   mul_2(f2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), new2));
           acc[ch * 16 + i] = lo_of(z), acc[ch * 16 + i + 1] = hi_of(z);
         }
       }
@@ -579,7 +599,10 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       if (lane == 0) mbar_arrive(&s.o_free[j & 1]);
     }
     ok = wait_for(&s.l_full, 0, error, 123) && ok;
-    const float by = inverse(s.l[y], ok);
+    float l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < SOFT; i++) l += s.l[i][y] * (s.m[i][y] == top ? 1.0f : ex2(s.m[i][y] - top));
+    const float by = inverse(l, ok);
 #pragma unroll
     for (int d = 0; d < HP; d += 8) {
       float z[8];
@@ -590,19 +613,20 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     write();
   } else {
     if (HALF) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    else if (SOFT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     // ---- the softmax of tile t_own. Its queries first, as float16 (float32: by a power of two into (0, 2), in two parts)
     // in the swizzled layout
-    const int t = t_own;
+    const int t = t_own, soft = SOFT == 2 ? (warp - BRINGERS / 32) >> 2 : 0;
     float qf = 1.0f;
-    s.row[t][y] = make_int2(on ? r.first + token : -1, head);
-    asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+    s.row[t][y] = make_int2(on ? r.first + token : -1, head);  // (SOFT 2: both warpgroups write, the same)
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + t + soft) : "memory");
     {
       // a row by LANES threads, 8 values each; ROWS rows' loads in flight
       constexpr int LANES = HP / 8, AT_ONCE = 128 / LANES, ROWS = HALF ? 8 : 4;
       const int col = y % LANES * 8, sub = y / LANES;
 #pragma unroll 1
-      for (int first = sub; first < QT; first += ROWS * AT_ONCE) {
+      for (int first = sub + soft * (QT / SOFT); first < (soft + 1) * (QT / SOFT); first += ROWS * AT_ONCE) {
         uint4 raw[ROWS][HALF ? 1 : 2];
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
@@ -628,7 +652,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
             for (int d = LANES / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
             const float f = __uint_as_float((uint32_t)(127 - e) << 23);
-            if (col == 0) s.l[row] = __uint_as_float((uint32_t)(127 + e) << 23);
+            if (col == 0) s.power[row] = __uint_as_float((uint32_t)(127 + e) << 23);
             uint32_t p[4], q[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -647,9 +671,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&s.q_full);
       if (!HALF) {
-        // the rows' powers of two, among the four warps (l is for the sums later)
-        asm volatile("bar.sync 3, 128;" ::: "memory");
-        qf = s.l[y];
+        asm volatile("bar.sync 3, %0;" ::"n"(128 * SOFT) : "memory");
+        qf = s.power[y];
       }
     }
     const int first_pos = r.length - r.fresh + (row0 + t * QT) / a.group;  // the tile's first row's
@@ -657,18 +680,18 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     float m = -INFINITY, l = 0.0f;
     const int n = steps[t];
     bool ok = true;
-    for (int j = 0; j < n && ok; j++) {
+    for (int j = soft; j < n && ok; j += SOFT) {
       // (the step's scales are there with its scores: the keys were complete before the scores were begun)
       ok = wait_for(&s.s_full[t][j % SBUF], (j / SBUF) & 1, error, 116);
       ok = wait_for(&s.kv_full[j % STAGES], (j / STAGES) & 1, error, 117) && ok;
       ok = __all_sync(0xffffffffu, ok);
       fence_after();
-      // where a row's maximum moves; by < 0: nowhere in the warp
+      // where a row's maximum moves, to m, and its sums go down by `by`; by < 0: nowhere in the warp
       auto settle = [&](float by) {
         if (!HALF) {
-          s.by[j & 3][y] = by < 0.0f ? 1.0f : by;
+          s.ref[j & 7][y] = m;
           __syncwarp();
-          if (lane == 0) mbar_arrive(&s.by_full[j & 3]);
+          if (lane == 0) mbar_arrive(&s.ref_full[j & 7]);
         } else if (by >= 0.0f && j > 0) {  // (whole warps come here: TMEM is read and written by whole warps)
           // O holds the steps so far: it goes to the new maxima once the last P V is done
           wait_for(&s.pv_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1, error, 109);
@@ -685,7 +708,6 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
             st8(o_col + ch * 16 + 8, o + 8);
           }
         }
-        return by;
       };
       // (rows that don't exist have pos -1: nothing of a step is theirs, and nothing of theirs is written)
       const uint32_t from = tS(t, j % SBUF) + lane_base;
@@ -697,7 +719,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       if (lane == 0) mbar_arrive(&s.p_full[t][j % SBUF]);
     }
     if (!HALF) {
-      s.l[y] = ok ? l : __uint_as_float(0x7fffffffu);
+      s.l[soft][y] = ok ? l : __uint_as_float(0x7fffffffu), s.m[soft][y] = m;
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.l_full);
     } else {
