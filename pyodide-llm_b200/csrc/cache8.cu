@@ -33,17 +33,21 @@ __device__ __forceinline__ int over(int x, int by, uint32_t inverse) {
 // for partial sums. Takes read the ring's live part and gives write behind it, takes write table entries that no
 // token's slot is read from (a token of a new block finds its id in the ring), so only lengths and state, which may
 // be updated in place, have to wait until every block has read them: the one cluster barrier.
-// Measured: 64 requests of a token each 6.8 us; 1000 that add 250 to 500 tokens each (358,000 slots) 22 us, of
-// which the running sums over 1000 requests and the barrier are most. A launch by itself is 2 to 3 us.
+// Steps of more than ROWS_APART rows have them written by a second launch, on all SMs: 1000 requests of 64 tokens each take
+// 14 us so and 20 with the cluster writing them, 64 of 512 8 and 9, 64 of 64 (the bound's other side) 8 by one block.
+// Measured: 64 requests of a token each 6.4 us; 1000 that add 250 to 500 tokens each (358,000 rows) 16.5 us, of which the
+// sums over 1000 requests, by every block, are most. A launch by itself is 2 to 3 us.
 
 constexpr int TT = 512;  // threads, and the requests of one tile of the running sums
+constexpr int ROWS_APART = 4096;  // a step's rows that the first launch writes at most
 
 struct Need {
   int64_t tokens, take, give;
 };
 
 // what request i asks for; `bad` collects B200K_TABLES_* of requests that cannot have it
-__device__ __forceinline__ Need need_of(int64_t length, int64_t add, int64_t most, int block, int &bad, int64_t &after) {
+__device__ __forceinline__ Need need_of(int64_t length, int64_t add, int64_t most, int block, uint32_t inverse, int &bad,
+                                        int64_t &after) {
   if (length < 0 || length > most) {
     bad |= 1 << B200K_TABLES_INPUT;
     after = length;
@@ -55,7 +59,7 @@ __device__ __forceinline__ Need need_of(int64_t length, int64_t add, int64_t mos
     bad |= 1 << B200K_TABLES_WIDTH;
     return {0, 0, 0};
   }
-  const int before_b = (int)((length + block - 1) / block), after_b = (int)((after + block - 1) / block);
+  const int before_b = over((int)length + block - 1, block, inverse), after_b = over((int)after + block - 1, block, inverse);
   return {add > 0 ? add : 0, after_b > before_b ? after_b - before_b : 0, before_b > after_b ? before_b - after_b : 0};
 }
 
@@ -84,6 +88,7 @@ struct TablesArgs {
   int32_t *tables, *ring, *state_out, *lengths_out, *starts, *slots, *seq, *pos;
   const int32_t *state, *lengths, *news;
   int n_seqs, width, blocks, block, n;
+  int apart;  // the tokens' rows are written by a kernel of their own
 };
 
 __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
@@ -109,7 +114,7 @@ __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
     length = 0;
     if (i < a.n_seqs) {
       length = a.lengths[i];
-      need = need_of(length, a.news[i], most, a.block, bad, after);
+      need = need_of(length, a.news[i], most, a.block, inverse, bad, after);
     }
     const int64_t own[3] = {need.tokens, need.take, need.give};
 #pragma unroll
@@ -132,10 +137,29 @@ __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
 
   // what everything comes to: all is granted, or nothing is
   int64_t sum[3] = {0, 0, 0};
-  for (int base = 0; base < a.n_seqs; base += TT) {
-    tile_of(base);
+  if (a.n_seqs <= TT) {
+    tile_of(0);
 #pragma unroll
-    for (int j = 0; j < 3; j++) sum[j] += all[j];
+    for (int j = 0; j < 3; j++) sum[j] = all[j];
+  } else {
+#pragma unroll 2
+    for (int i = tid; i < a.n_seqs; i += TT) {
+      const Need one = need_of(a.lengths[i], a.news[i], most, a.block, inverse, bad, after);
+      sum[0] += one.tokens, sum[1] += one.take, sum[2] += one.give;
+    }
+#pragma unroll
+    for (int j = 0; j < 3; j++) {
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], d);
+      if (lane == 0) part[j][warp] = sum[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 3; j++) {
+      sum[j] = 0;
+#pragma unroll
+      for (int w = 0; w < TT / 32; w++) sum[j] += part[j][w];
+    }
   }
   bad = __syncthreads_or(bad & 1 << B200K_TABLES_INPUT) ? 1 << B200K_TABLES_INPUT
         : __syncthreads_or(bad & 1 << B200K_TABLES_WIDTH) ? 1 << B200K_TABLES_WIDTH : 0;
@@ -167,7 +191,7 @@ __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
       // the tokens of this tile of requests, their slots from the table or, in blocks taken now, from the ring; a few of
       // them at a time, so that their lookups overlap
       constexpr int AT_ONCE = 4;
-      for (int t0 = carry[0] + first; t0 < sums[0][TT]; t0 += AT_ONCE * stride) {
+      for (int t0 = a.apart ? sums[0][TT] : carry[0] + first; t0 < sums[0][TT]; t0 += AT_ONCE * stride) {
         int s[AT_ONCE], p[AT_ONCE], id[AT_ONCE], b[AT_ONCE];
 #pragma unroll
         for (int k = 0; k < AT_ONCE; k++) s[k] = find(sums[0], tile, min(t0 + k * stride, sums[0][TT] - 1));
@@ -205,7 +229,7 @@ __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
   }
   if (rank == 0 && tid == 0) a.starts[a.n_seqs] = total;
   // rows of the step's buffers behind its tokens
-  for (int t = total + first; t < a.n; t += stride) {
+  for (int t = a.apart ? a.n : total + first; t < a.n; t += stride) {
     a.slots[t] = -1;
     if (a.seq) a.seq[t] = -1;
     if (a.pos) a.pos[t] = -1;
@@ -217,7 +241,7 @@ __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
     if (a.n_seqs > TT || ranks > 1) {
       length = a.lengths[i];
       int none = 0;
-      need_of(length, a.news[i], most, a.block, none, after);
+      need_of(length, a.news[i], most, a.block, inverse, none, after);
     }
     a.lengths_out[i] = granted ? (int)after : length;
   }
@@ -231,6 +255,46 @@ __global__ void __launch_bounds__(TT) block_tables_kernel(TablesArgs a) {
     a.state_out[1] = granted ? (int)(count - sum[1] + sum[2]) : count;
     a.state_out[2] = status;
     a.state_out[3] = total;
+  }
+}
+
+// The rows of a step of many tokens, from what block_tables_kernel has written: a warp takes CHUNK of them side by side,
+// finds the first one's request in the running sums, the last one's, and each token's between them.
+constexpr int RT_THREADS = 256, CHUNK = 128;
+__global__ void __launch_bounds__(RT_THREADS) block_rows_kernel(TablesArgs a) {
+  pdl_begin();
+  const int lane = threadIdx.x & 31, t0 = (blockIdx.x * (RT_THREADS / 32) + (threadIdx.x >> 5)) * CHUNK;
+  if (t0 >= a.n) return;
+  const int total = a.starts[a.n_seqs], last = min(t0 + CHUNK, total) - 1;
+  const uint32_t inverse = inverse_of(a.block);
+  // the request whose rows hold t, of those from lo to hi (none below hi starts behind t)
+  auto request_of = [&](int t, int lo, int hi) {
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.starts[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
+  int low = 0, high = 1;
+  if (t0 < total) {
+    low = request_of(t0, 0, a.n_seqs);
+    high = last < a.starts[low + 1] ? low + 1 : request_of(last, low, a.n_seqs) + 1;
+  }
+#pragma unroll
+  for (int k = 0; k < CHUNK / 32; k++) {
+    const int t = t0 + 32 * k + lane;
+    if (t >= a.n) return;
+    int slot = -1, s = -1, p = -1;
+    if (t < total) {
+      s = request_of(t, low, high);
+      p = a.lengths_out[s] - (a.starts[s + 1] - t);
+      const int b = over(p, a.block, inverse), id = a.tables[(int64_t)s * a.width + b];
+      if (id >= 0 && id < a.blocks) slot = id * a.block + (p - b * a.block);
+    }
+    a.slots[t] = slot;
+    if (a.seq) a.seq[t] = s;
+    if (a.pos) a.pos[t] = p;
   }
 }
 
@@ -573,7 +637,7 @@ extern "C" int b200k_block_tables(int32_t *tables, int32_t *ring, int32_t *state
         (int64_t)table_width * block > INT32_MAX / 2)
       return fail(B200FWD_EINVAL, "block_tables: 1 block at least, and positions and slots that an int32 holds");
     TablesArgs a = {tables, ring, state_out, lengths_out, starts, slots, seq, pos, state, lengths, news,
-                    n_seqs, table_width, blocks, block, n};
+                    n_seqs, table_width, blocks, block, n, n > ROWS_APART};
     // one block up to 4096 tokens and 2 tiles of requests, else a cluster of eight
     const unsigned ranks = n <= 4096 && n_seqs <= 2 * TT ? 1 : 8;
     cudaLaunchAttribute attr[2];
@@ -590,6 +654,11 @@ extern "C" int b200k_block_tables(int32_t *tables, int32_t *ring, int32_t *state
     cfg.numAttrs = pdl_on() ? 2 : 1;
     (void)cudaLaunchKernelEx(&cfg, block_tables_kernel, a);
     B200_LAUNCHED("block_tables");
+    if (a.apart) {
+      const int per_block = RT_THREADS / 32 * CHUNK;
+      launch(block_rows_kernel, dim3((n + per_block - 1) / per_block), dim3(RT_THREADS), 0, as_stream(stream), a);
+      B200_LAUNCHED("block_rows");
+    }
     return 0;
   } catch (...) {
     return fail(B200FWD_EINVAL, "block_tables: exception");

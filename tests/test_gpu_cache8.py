@@ -91,6 +91,19 @@ def test_block_tables_follow_the_requests(S, width, block, most, seed):
     assert granted >= 2
 
 
+@pytest.mark.parametrize("n", [4095, 4096, 4097, 5000, 9001])
+def test_block_tables_of_many_rows(n):
+    """Steps around the rows from which another kernel writes them: requests without tokens among long ones and at both
+    ends, a request that ends a step's rows, steps that are not granted, blocks' ends between two warps' rows."""
+    rng = np.random.default_rng(n)
+    d = DeviceTables(plain.Tables(9, 700, 700, 16, 690, rng.permutation(700)))
+    assert same_step(d, [0, 0, 1500, 1, 0, n - 1503, 0, 2, 0], n) == 0
+    assert same_step(d, [3, -1500, 0, 1, 0, 11200, 0, 0, 0], n) == abi.TABLES_WIDTH
+    assert same_step(d, [3, -1500, 0, 1, 0, 0, 0, n, 0], n) == abi.TABLES_TOKENS
+    assert same_step(d, [1, -2 ** 31, -2 ** 31, 0, 0, -2 ** 31, 129, 127, 0], n, with_rows=False) == 0
+    assert same_step(d, [0, 128, 0, 0, 1, 0, 0, 0, 4000], n, out_of_place=True) == (0 if n >= 4129 else abi.TABLES_TOKENS)
+
+
 def test_block_tables_grant_all_or_nothing():
     d = DeviceTables(plain.Tables(3, 4, 6, 16, 2, [5, 1, 3, 0, 2, 4]))
     assert same_step(d, [17, 16, 1], 34) == 0                      # four of six blocks
