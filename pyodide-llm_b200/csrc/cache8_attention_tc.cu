@@ -4,7 +4,8 @@
 //
 // A thread block takes 256 (float16) or 128 (float32) rows of one request and kv head, in tiles of 128 (row x: query head
 // x % group of the request's token x / group, so the heads that share a kv head share its keys), and walks their
-// positions in steps of 64. 640 threads:
+// positions in steps of 64. 640 threads (float32 with heads of up to 64: warps 0..3 bring the cache, and warps 4..7 and 8..11
+// are the softmax of even and of odd steps, each with a running maximum and sum of its own):
 //   warps 0..7 bring the cache: int8 keys and values by 16-byte loads one step ahead, widened to float16 (exact) into
 //     shared memory in the tensor cores' 128-byte swizzled layout; a step's four units' scales beside them. Positions
 //     are rows of both: for K Q^T they run along N, for P V along K, and the values' operand is described as major along
@@ -19,9 +20,10 @@
 // What bounds it, in cycles. Float16, heads of 128: a step of both tiles takes 2330, of which the products are 1540 (S with
 // its N of 64 at half rate: 63 for each 16 of K, as Q comes from shared memory every time; P V 66), exponentials 1024,
 // issue slots 1400; a block begins and ends in 15,000 (the queries, the first keys, the first scores; rows out) beside 30
-// steps on average. Float32, heads of 64: 2060 a step, one after the other a row's scores, weights and their two parts.
+// steps on average. Float32, heads of 64: 1550 a step of one tile (one warpgroup of softmax: 2060), of which the products
+// are about 900; each softmax step takes 2300 to 2600, twice its instructions' issue slots.
 // Measured: 8 requests that add 260 to 509 tokens to contexts of up to 4500, 32 query and 8 kv heads of 128, float16: 172 us
-// (0.64 PFLOP/s of what the masks leave); 4 whole prompts of 2048 tokens, 8 heads of 64, float32: 97 us.
+// (0.64 PFLOP/s of what the masks leave); 4 whole prompts of 2048 tokens, 8 heads of 64, float32: 87 us.
 // TMEM (512 columns), float16: tile t's two score buffers at 128 t + {0, 64}, its O at 256 + t * head size; float32: three
 // score buffers at {0, 64, 128}, two of O at 192 + {0, 1} * head size.
 // Every wait is bounded: past it the kernel sets the scratch's error word and runs to its end.
