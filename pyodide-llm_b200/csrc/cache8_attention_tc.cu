@@ -25,7 +25,7 @@
 // Measured: 8 requests that add 260 to 509 tokens to contexts of up to 4500, 32 query and 8 kv heads of 128, float16: 172 us
 // (0.64 PFLOP/s of what the masks leave); 4 whole prompts of 2048 tokens, 8 heads of 64, float32: 87 us.
 // TMEM (512 columns), float16: tile t's two score buffers at 128 t + {0, 64}, its O at 256 + t * head size; float32: three
-// score buffers at {0, 64, 128}, two of O at 192 + {0, 1} * head size.
+// score buffers (heads of up to 64: four) at 64 u, two of O behind them.
 // Every wait is bounded: past it the kernel sets the scratch's error word and runs to its end.
 #include <string>
 
