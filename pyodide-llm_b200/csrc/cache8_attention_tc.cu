@@ -54,7 +54,7 @@ struct Tc {
     alignas(1024) uint8_t q[TILES][PARTS][CHUNKS][QT * 128];
     alignas(1024) uint8_t k[STAGES][CHUNKS][KT * 128];
     alignas(1024) uint8_t v[STAGES][CHUNKS][KT * 128];
-    alignas(16) float4 sc[STAGES][KU];  // a unit's {key scale * log2(e) / sqrt(hs), log2(value scale), 1 / value scale}
+    alignas(16) float4 sc[STAGES][KU];  // a unit's {key scale, log2(value scale), 1 / value scale}
     // float32: the maxima that a step's weights are relative to (softmax is up to SBUF + 1 steps ahead of the sums); at the
     // end each warpgroup's sums and maxima; the powers of two that the queries were divided by
     float ref[8][QT], l[SOFT][QT], m[SOFT][QT], power[QT];
@@ -193,8 +193,8 @@ __device__ __forceinline__ float lo_of(uint64_t v) { return __uint_as_float((uin
 __device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
 // One step of this thread's row: 64 scores from tS, their weights over them. EDGE: some of the tile's rows don't see all
-// of the step; limit: the last position that this row sees, from the step's first. m, l: the row's running maximum and
-// sum. settle(by): called by the whole warp once m is settled, where some row's maximum moved with what the
+// of the step; limit: the last position that this row sees, from the step's first. qf: what a score takes besides its key
+// scale, log2(e) / sqrt(hs) and the power of two that the row was divided by. m, l: the row's running maximum and sum. settle(by): called by the whole warp once m is settled, where some row's maximum moved with what the
 // row's sums go down by. (The next step's scores, loaded while this one's last weights are worked out, cost more than they saved: 189
 // us for 172, 102 for 97.)
 template <int HP, bool HALF, bool EDGE, typename Settle>
@@ -210,6 +210,8 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, const float4 *sc, floa
     c[u] = s.x * qf, lg[u] = s.y, inv[u] = s.z;
     // (a unit that the row does not see may have any scales, NaN too)
     if (EDGE && u * UNIT > limit) c[u] = 1.0f, lg[u] = 0.0f, inv[u] = 0.0f;
+    // (a factor of 0, of a row or keys of zeros, as the least, which moves no exponent: 0 times a masked -inf is no number)
+    if (EDGE && c[u] < 1e-30f) c[u] = 1e-30f;
   }
   wait_ld32(x);
   wait_ld32(x + 32);
@@ -486,9 +488,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
         forward(far[i]);
       }
       if (tid < KU) {
-        // a key scale of 0 (a block of zeros) as the least: 0 times a masked -inf is no number
-        const float c = !(ks * a.scale < 1e-30f) ? ks * a.scale : 1e-30f, w = !(vs < LEAST) ? vs : LEAST;
-        s.sc[slot][tid] = make_float4(c, __log2f(w), reciprocal(w), 0.0f);
+        const float w = !(vs < LEAST) ? vs : LEAST;
+        s.sc[slot][tid] = make_float4(ks, __log2f(w), reciprocal(w), 0.0f);
         if (more) {
           scales(spage);
           spage = page_of(sfar);
@@ -620,7 +621,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     // ---- the softmax of tile t_own. Its queries first, as float16 (float32: by a power of two into (0, 2), in two parts)
     // in the swizzled layout
     const int t = t_own, soft = SOFT == 2 ? (warp - BRINGERS / 32) >> 2 : 0;
-    float qf = 1.0f;
+    float qf = a.scale;
     s.row[t][y] = make_int2(on ? r.first + token : -1, head);  // (SOFT 2: both warpgroups write, the same)
     asm volatile("bar.sync %0, 128;" ::"r"(1 + t + soft) : "memory");
     {
@@ -674,7 +675,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       mbar_arrive(&s.q_full);
       if (!HALF) {
         asm volatile("bar.sync 3, %0;" ::"n"(128 * SOFT) : "memory");
-        qf = s.power[y];
+        qf = s.power[y] * a.scale;
       }
     }
     const int first_pos = r.length - r.fresh + (row0 + t * QT) / a.group;  // the tile's first row's

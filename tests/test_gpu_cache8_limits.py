@@ -1,0 +1,38 @@
+"""Where the paged 8-bit cache and its attention can go wrong: queries and keys of zeros, queries of any size, scales at
+float32's lower end, starts that do not ascend, outliers among a query's values, weights far below the largest one, and
+requests of more steps than the prompt kernel's rings hold. GPU only."""
+import numpy as np
+import pytest
+
+from test_gpu_cache8 import Case
+
+pytestmark = pytest.mark.gpu
+
+# more than 64 rows a kv head and heads of up to 128: the prompt kernel
+PROMPTS = [(150, 150), (90, 70), (200, 129)]
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("hs", [48, 64, 128])
+@pytest.mark.parametrize("size", [0.0, 1e-38, 1e-16])
+def test_prompts_of_zero_queries_and_keys(size, hs, half):
+    """Rows of zeros (or hardly more) over keys of zeros: every visible position weighs the same. Keys whose scale is so
+    small that its product with the row's is no float32, and ordinary ones, beside them."""
+    c = Case(PROMPTS, 2, 1, hs, 16, half, seed=hs)
+    c.q *= size
+    for page in c.tables[0, :10]:
+        c.kc[page], c.ks[page] = 0, 0
+    c.ks[c.tables[1, :6]] = 1e-9
+    got = c.run()
+    assert np.isfinite(got).all()
+    c.check(got)
+
+
+@pytest.mark.parametrize("hs", [48, 64, 128])
+@pytest.mark.parametrize("size", [1e-30, 1e25, 1e37])
+def test_prompts_of_queries_of_any_size(size, hs):
+    """float32 queries far outside float16's range, over keys that bring their scores back: scores stay as exact."""
+    c = Case(PROMPTS, 2, 2, hs, 16, False, seed=8)
+    c.q *= size
+    c.ks *= np.float32(1 / size if size < 1e30 else 1e-37)
+    c.check(c.run())
