@@ -323,10 +323,10 @@ int b200k_block_tables(int32_t *tables, int32_t *ring, int32_t *state_out, int32
 /* Keys and values k, v (n rows of nkv * hs, k_stride and v_stride elements apart) into their slots; rows with a slot
  * that is none are left out. A block's tokens stand next to one another in the call, in the order of their slots, each
  * slot once. A (block, head)'s scale is the float32 nearest to max |x| / 127 over all its values (earlier ones by the
- * scale that they had), the integers are nearest to x / scale, half to even. Positions before the first one stored now
- * are the block's earlier tokens: where the scale grows, their integers go to the new step the same way, q * old / new.
- * Storing position 0 of a block begins it anew. A value that is no finite number makes the (block, head)'s scale NaN
- * and its new integers 0: it reads as NaN until the block is begun anew. */
+ * scale that they had), the integers are nearest to x / scale, half to even, and from -127 to 127. Positions before the
+ * first one stored now are the block's earlier tokens: where the scale grows, their integers go to the new step the same
+ * way, q * old / new. Storing position 0 of a block begins it anew. A value that is no finite number makes the (block,
+ * head)'s scale NaN and its new integers 0: it reads as NaN until the block is begun anew. */
 int b200k_cache8_store(int8_t *kc, float *ks, int8_t *vc, float *vs, const void *k, const void *v,
                        const int32_t *slots, int32_t n, int64_t k_stride, int64_t v_stride, int32_t blocks,
                        int32_t block, int32_t nkv, int32_t hs, int32_t half, b200fwd_stream stream);

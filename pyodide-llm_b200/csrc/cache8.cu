@@ -329,8 +329,10 @@ __device__ __forceinline__ void values_of(const uint4 &u, float (&x)[8]) {
 }
 
 // the integer nearest to q a / b, half to even, in 64 bits: q a is exact there (q an integer of 8 bits, or 1 and a a
-// float), and so far from a half that is not one that the quotient's rounding cannot reach it
-__device__ __noinline__ int exactly(double qa, double b) { return (int)rint(__ddiv_rn(qa, b)); }
+// float), and so far from a half that is not one that the quotient's rounding cannot reach it. At most 127 in size: a
+// scale of a few of float32's smallest steps may be a third below the largest value's 127th part (and has no inverse, so
+// all its values come here).
+__device__ __noinline__ int exactly(double qa, double b) { return (int)fmin(fmax(rint(__ddiv_rn(qa, b)), -127.0), 127.0); }
 
 // the largest |x|: NaN above infinity above every number
 __device__ __forceinline__ float max_nan(float a, float b) {

@@ -69,7 +69,7 @@ def store(cache, scales, x, slots, block):
                 cache[page, h, :held] = np.rint(cache[page, h, :held].astype(np.float64) * np.float64(old) / np.float64(new))
             for t in range(m):
                 q = np.rint(run[t] / np.float64(new)) if new > 0 else np.zeros(run.shape[1])
-                cache[page, h, slots[i + t] % block] = q
+                cache[page, h, slots[i + t] % block] = np.clip(q, -127, 127)  # (of the smallest scales up to 190)
         i += m
 
 

@@ -4,7 +4,7 @@ requests of more steps than the prompt kernel's rings hold. GPU only."""
 import numpy as np
 import pytest
 
-from test_gpu_cache8 import Case
+from test_gpu_cache8 import Case, store_case
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +36,16 @@ def test_prompts_of_queries_of_any_size(size, hs):
     c.q *= size
     c.ks *= np.float32(1 / size if size < 1e30 else 1e-37)
     c.check(c.run())
+
+
+def test_store_of_the_smallest_scales():
+    """float32 scales of one to seven of its smallest steps: the largest value may be up to 190 of them, and is stored as
+    127, of its own sign."""
+    step = 2.0 ** -149
+    largest = np.array([64, 100, 127, 150, 190, 191, 260, 317, 318, 400, 700, 889])
+    x = np.linspace(-1, 1, 32) * (largest * step)[:, None]
+    (kc, ks), (vc, _) = store_case(x[:, None], -x[:, None], np.arange(12) * 16, 12, 16, 1, 32, False, 1)
+    assert ks[4, 0] == np.float32(step) and (kc[4, 0, 0, [0, -1]] == [-127, 127]).all()
+    for cache in (kc, vc):
+        x32 = x.astype(np.float32).astype(np.float64) * (1 if cache is kc else -1)
+        assert (np.sign(cache[:, 0, 0]) * np.sign(x32) >= 0).all()
