@@ -366,7 +366,8 @@ __device__ __forceinline__ uint32_t four_bytes(const float *x, float s, float in
   }
   return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
-// four earlier integers from scale a to scale b, ratio about a / b (q a is rounded here: by 2^-24 of 127 b at most)
+// four earlier integers from scale a to scale b, ratio about a / b (q a is rounded here: by 2^-24 of 127 b at most; where b
+// is a few of float32's smallest steps the margin rounds to b itself, and a tie has to be let through)
 __device__ __forceinline__ uint32_t four_moved(uint32_t q4, float a, float b, float ratio) {
   float off = 0.0f;
   uint32_t t[4];
@@ -376,7 +377,7 @@ __device__ __forceinline__ uint32_t four_moved(uint32_t q4, float a, float b, fl
     t[j] = __float_as_uint(z);
     off = fmaxf(off, fabsf(__fmaf_rn(-(z - 12582912.0f), b, __fmul_rn(q, a))));
   }
-  if (off + off > b * 0.99997f) {
+  if (off + off >= b * 0.99997f) {
 #pragma unroll 1
     for (int j = 0; j < 4; j++) t[j] = (uint32_t)exactly((double)(int8_t)(q4 >> (8 * j)) * a, b);
   }

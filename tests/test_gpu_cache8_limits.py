@@ -49,3 +49,16 @@ def test_store_of_the_smallest_scales():
     for cache in (kc, vc):
         x32 = x.astype(np.float32).astype(np.float64) * (1 if cache is kc else -1)
         assert (np.sign(cache[:, 0, 0]) * np.sign(x32) >= 0).all()
+
+
+def test_store_moves_the_smallest_scales():
+    """A block whose scale goes from 1, 2, ... of float32's smallest steps to a few more: earlier integers that fall on a half
+    go to the even one."""
+    step = 2.0 ** -149
+    n, hs = 9, 128
+    x = np.tile(np.arange(128) - 64.0, (n, 1)) * step
+    x[:, 0] = 127 * (1 + np.arange(n)) * step
+    kv = store_case(x[:, None], -x[:, None], np.arange(n) * 16, n, 16, 1, hs, False, 1)
+    y = np.zeros((n, hs))
+    y[:, 0] = 127 * 6 * step * (1 + np.arange(n) // 3)
+    store_case(y[:, None], -y[:, None], np.arange(n) * 16 + 1, n, 16, 1, hs, False, 1, kv=kv)
