@@ -106,7 +106,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return y;
 }
 
-// sums of {work, tiles, new tokens} over the requests before this thread's (one request a thread), and of all
+// sums of {work, tiles, requests astray} over the requests before this thread's (one request a thread), and of all
 __device__ __forceinline__ void block_scan(int64_t (&v)[3], int64_t (&all)[3], int64_t (*part)[WARPS]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t own[3] = {v[0], v[1], v[2]};
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
     v[0] = v[1] = v[2] = w = 0;
     if (i < a.n_seqs) {
       const Request r = request_of(a, i);
-      v[2] = r.fresh;
+      v[2] = r.astray;
       v[1] = tiles_of<RT>(a, r);
       w = v[0] = v[1] * (a.whole_tiles ? 1 : units_of(a, r));
     }
@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
 #pragma unroll
     for (int j = 0; j < 3; j++) sum[j] += all[j];
   }
-  // (starts that don't ascend: rows of several requests, nothing is written)
-  const int64_t total = sum[2] > a.n ? 0 : sum[0];
+  // (starts that don't ascend: nothing is written)
+  const int64_t total = sum[2] ? 0 : sum[0];
   const int64_t span = max((int64_t)a.min_work, (total + gridDim.x - 1) / gridDim.x);
   int64_t at = span * blockIdx.x;
   const int64_t end = min(at + span, total);

@@ -31,13 +31,15 @@ struct Args {
   float scale;      // log2(e) / sqrt(hs)
 };
 
-// request i of the call: its first row, its rows, and its positions (all of them, the new ones included)
+// request i of the call: its first row, its rows, and its positions (all of them, the new ones included); astray: its
+// starts do not ascend within 0..n (the whole call then writes nothing; the rows given here are in bounds all the same)
 struct Request {
   int first, fresh, length;
+  bool astray;
 };
 __device__ __forceinline__ Request request_of(const Args &a, int i) {
-  const int s0 = min(max(a.starts[i], 0), a.n), s1 = min(max(a.starts[i + 1], s0), a.n);
-  return {s0, s1 - s0, max(a.lengths[i], 0)};
+  const int at = a.starts[i], to = a.starts[i + 1], s0 = min(max(at, 0), a.n), s1 = min(max(to, s0), a.n);
+  return {s0, s1 - s0, max(a.lengths[i], 0), s0 != at || s1 != to};
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) {

@@ -274,14 +274,15 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
 
   // ---- which request's which group of TILES tiles: a request's last rows, which see the most positions, first, and up to
   // SORTED requests the longest first (a block's time is its positions'; what starts last should be short)
-  int total = 0, fresh = 0;
+  int total = 0, astray = 0;
   if (tid == 0) s.found[0] = -1;
   for (int base = 0; base < a.n_seqs; base += THREADS) {
     const int i = base + tid;
-    int groups = 0, own = 0;
+    int groups = 0;
+    bool own = false;
     if (i < a.n_seqs) {
       const Request r = request_of(a, i);
-      own = r.fresh;
+      own = r.astray;
       groups = r.fresh * a.group > a.rows_most ? (r.fresh * a.group + TILES * QT - 1) / (TILES * QT) : 0;
       if (a.n_seqs <= SORTED) s.of[tid] = make_int2(r.length, groups);
     }
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       const int o = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += o;
     }
-    own = __reduce_add_sync(0xffffffffu, own);
+    own = __any_sync(0xffffffffu, own);
     __syncthreads();
     if (lane == 31) s.part[0][warp] = upto, s.part[1][warp] = own;
     __syncthreads();
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     for (int w = 0; w < min(THREADS / 32, (a.n_seqs - base + 31) / 32); w++) {
       if (w < warp) before += s.part[0][w];
       total += s.part[0][w];
-      fresh = min(fresh + s.part[1][w], a.n + 1);
+      astray |= s.part[1][w];
     }
     before += upto - groups;
     if (a.n_seqs <= SORTED && i < a.n_seqs) {
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     const int x = index - before;
     if (x >= 0 && x < groups) s.found[0] = i, s.found[1] = groups - 1 - x;
   }
-  if (fresh > a.n) return;  // starts that don't ascend
+  if (astray) return;  // starts that don't ascend
   __syncthreads();
   const int req = s.found[0];
   if (req < 0) return;

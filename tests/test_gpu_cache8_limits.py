@@ -4,6 +4,7 @@ requests of more steps than the prompt kernel's rings hold. GPU only."""
 import numpy as np
 import pytest
 
+from gpu_util import host
 from test_gpu_cache8 import Case, store_case
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +63,35 @@ def test_store_moves_the_smallest_scales():
     y = np.zeros((n, hs))
     y[:, 0] = 127 * 6 * step * (1 + np.arange(n) // 3)
     store_case(y[:, None], -y[:, None], np.arange(n) * 16 + 1, n, 16, 1, hs, False, 1, kv=kv)
+
+
+@pytest.mark.parametrize("starts,requests", [
+    ([0, 5, 2, 7], [(50, 3), (50, 2), (50, 2)]), ([3, -4, 9, 1000], [(50, 3), (50, 2), (50, 2)]),
+    ([0, 5, 3, 5], [(50, 3), (50, 2), (50, 2)]), ([0, 1, 2, 8], [(50, 3), (50, 2), (50, 2)]),
+    ([-1, 2, 4, 6], [(900, 3), (50, 2), (50, 2)]), ([4, 4, 3, 3], [(900, 3), (50, 2), (50, 2)]),
+    ([0, 100, 90, 300], [(200, 100), (150, 100), (700, 100)]), ([0, 100, 200, 301], [(200, 100), (150, 100), (700, 100)]),
+    ([-2 ** 31, 100, 200, 300], [(200, 100), (150, 100), (700, 100)])])
+@pytest.mark.parametrize("half", [False, True])
+def test_attention_writes_nothing_where_starts_do_not_ascend(starts, requests, half):
+    """starts that go down, begin below 0 or end behind the call's rows: no row is written, few rows and prompts, short
+    tables and long ones."""
+    c = Case(requests, 4, 2, 64, 16, half, seed=5)
+    c.starts, c.behind = np.array(starts), 0
+    c.upload()
+    c.dq_wide = c.dq
+    c.call()
+    assert (host(c.out) == 7).all()
+
+
+@pytest.mark.parametrize("at", [0, 127, 128, 640, 699])
+def test_attention_finds_starts_that_do_not_ascend_among_many(at):
+    """One pair of starts out of order among 700 requests, in any of the parts in which the kernels look them over."""
+    c = Case([(30, 1)] * 699 + [(200, 150)], 4, 2, 64, 16, False, seed=6)
+    c.behind = 0
+    good = c.run()
+    c.check(good)
+    c.starts[at] = c.starts[at + 1] + 1 if at else -1
+    c.upload()
+    c.dq_wide = c.dq
+    c.call()
+    assert (host(c.out) == 7).all()
