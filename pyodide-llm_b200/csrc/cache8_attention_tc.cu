@@ -698,8 +698,9 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
           if (lane == 0) mbar_arrive(&s.ref_full[j & 7]);
         } else if (by >= 0.0f && j > 0) {  // (whole warps come here: TMEM is read and written by whole warps)
           // O holds the steps so far: it goes to the new maxima once the last P V is done
-          wait_for(&s.pv_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1, error, 109);
-          __syncwarp();
+          // (given up: O stays as it is, and the rows come out NaN)
+          ok = __all_sync(0xffffffffu, wait_for(&s.pv_done[t][(j - 1) & 1], ((j - 1) >> 1) & 1, error, 109)) && ok;
+          if (!ok) return;
           fence_after();
 #pragma unroll
           for (int ch = 0; ch < HP / 16; ch++) {
