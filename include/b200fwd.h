@@ -352,6 +352,9 @@ int b200k_cache8_attention(void *out, const void *q, const int8_t *kc, const flo
                            b200fwd_stream stream);
 int b200k_cache8_attention_scratch(int32_t n, int32_t n_seqs, int32_t nh, int32_t nkv, int32_t hs, int32_t half,
                                    uint64_t *bytes);
+/* b200k_cache8_attention only enqueues its kernels; this waits for the last call with this scratch and gives
+ * B200FWD_ETIMEOUT where one of the kernels' bounded waits gave up in it (the rows it concerns are NaN), else 0. */
+int b200k_cache8_attention_check(const void *scratch, b200fwd_stream stream);
 /* What a sampler's answer is reported with, of `count` rows of n logits (stride elements apart; float16 where half):
  * logprob[r] = log softmax(row r)[targets[r]] (NaN where the target is no id; NULL: not wanted), entropy[r] = -sum p log p
  * in nats (NULL: not wanted), and the k (0 to 32) most probable ids with their log probabilities, top_id and top_logprob

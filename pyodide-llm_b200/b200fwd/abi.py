@@ -177,6 +177,7 @@ def load():
         "b200k_cache8_attention": (P, P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, I32, I32, I32, I64, I64, I32, P,
                                    P),
         "b200k_cache8_attention_scratch": (I32, I32, I32, I32, I32, I32, ctypes.POINTER(U64)),
+        "b200k_cache8_attention_check": (P, P),
         "b200k_logprobs": (P, P, P, P, P, P, I32, I32, I64, I32, I32, P),
     }
     for name, args in sig.items():

@@ -810,6 +810,20 @@ extern "C" int b200k_cache8_attention_scratch(int32_t n, int32_t n_seqs, int32_t
   }
 }
 
+extern "C" int b200k_cache8_attention_check(const void *scratch, b200fwd_stream stream) {
+  try {
+    if (!scratch || reinterpret_cast<uintptr_t>(scratch) % 256)
+      return fail(B200FWD_EINVAL, "cache8_attention_check: scratch must be 256-byte aligned, and not null");
+    int32_t code = 0;  // (Args::meta[-1].y)
+    B200_CUDA(cudaMemcpyAsync(&code, reinterpret_cast<const int32_t *>(scratch) + 1, 4, cudaMemcpyDeviceToHost, as_stream(stream)));
+    B200_CUDA(cudaStreamSynchronize(as_stream(stream)));
+    if (code) return fail(B200FWD_ETIMEOUT, "cache8_attention: a pipeline wait gave up (code " + std::to_string(code) + ")");
+    return 0;
+  } catch (...) {
+    return fail(B200FWD_EINVAL, "cache8_attention_check: exception");
+  }
+}
+
 extern "C" int b200k_cache8_attention(void *out, const void *q, const int8_t *kc, const float *ks, const int8_t *vc,
                                       const float *vs, const int32_t *tables, const int32_t *starts,
                                       const int32_t *lengths, int32_t n, int32_t n_seqs, int32_t table_width,

@@ -26,7 +26,7 @@
 // (0.64 PFLOP/s of what the masks leave); 4 whole prompts of 2048 tokens, 8 heads of 64, float32: 87 us.
 // TMEM (512 columns), float16: tile t's two score buffers at 128 t + {0, 64}, its O at 256 + t * head size; float32: three
 // score buffers (heads of up to 64: four) at 64 u, two of O behind them.
-// Every wait is bounded: past it the kernel sets the scratch's error word and runs to its end.
+// Every wait is bounded: past it the kernel sets the scratch's error word (b200k_cache8_attention_check) and runs to its end.
 #include <string>
 
 #include "cache8_attention.cuh"

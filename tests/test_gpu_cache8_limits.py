@@ -4,7 +4,8 @@ requests of more steps than the prompt kernel's rings hold. GPU only."""
 import numpy as np
 import pytest
 
-from gpu_util import host
+from b200fwd import abi
+from gpu_util import host, ptr
 from test_gpu_cache8 import Case, store_case
 
 pytestmark = pytest.mark.gpu
@@ -95,3 +96,17 @@ def test_attention_finds_starts_that_do_not_ascend_among_many(at):
     c.dq_wide = c.dq
     c.call()
     assert (host(c.out) == 7).all()
+
+
+def test_attention_check_reads_the_scratch():
+    """0 after a call, whatever the scratch held before it; the error that a kernel's wait would leave there (planted by the
+    host here) as B200FWD_ETIMEOUT, until the next call."""
+    lib = abi.load()
+    c = Case([(200, 150), (90, 1)], 4, 2, 64, 16, False, seed=7)
+    c.run()
+    assert lib.b200k_cache8_attention_check(ptr(c.scratch), None) == 0
+    c.scratch[1] = 104
+    assert lib.b200k_cache8_attention_check(ptr(c.scratch), None) == abi.ETIMEOUT
+    assert "104" in abi.last_error()
+    c.call()
+    assert lib.b200k_cache8_attention_check(ptr(c.scratch), None) == 0
