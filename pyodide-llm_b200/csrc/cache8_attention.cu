@@ -9,9 +9,10 @@
 //  - scores: the keys' bytes as they are (m16n8k32, signed bytes, exact int32 sums) with the queries in fixed point, each
 //    row by a power of two into (0, 2) and then as three digits of a byte, 21 bits behind the point: a column for each
 //    digit of each row, whose sums are put together in float32.
-//  - values: as float16 integers (exact), with the weights as a float16 pair high + low (float16 queries: one float16, half
-//    a step of the output's type).
-//  - weights: w = 2^(s + log2(vscale) - M), M a running maximum (per row) that moves only when it is passed by more
+//  - values: as float16 integers (exact), with the weights as a float16 pair high + low / 2^11, the low part taken so far up
+//    that it keeps its 11 bits down to 2^-43 of the largest weight (float16 queries: one float16, half a step of the
+//    output's type, down to 2^-31 of the largest).
+//  - weights: w = 2^(s + log2(vscale) - M + 7), M a running maximum (per row) that moves only when it is passed by more
 //    than 2^8, and the row sum l += w / vscale: the block's value scale costs no operation per value, and what is
 //    rounded to float16 is relative to the largest term of the sum, whatever the scales.
 // Work is split over the length of the caches: the tiles' units of 16 positions, laid end to end, are cut into equal
@@ -99,6 +100,11 @@ __device__ __forceinline__ void query(const void *q, int64_t at, float (&z)[4]) 
     const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(q) + at);
     z[0] = v.x, z[1] = v.y, z[2] = v.z, z[3] = v.w;
   }
+}
+// two float16 integers times 2^-11
+__device__ __forceinline__ uint32_t lowered(uint32_t x) {
+  const __half2 v = __hmul2(*reinterpret_cast<const __half2 *>(&x), __half2half2(__ushort_as_half(0x1000)));
+  return *reinterpret_cast<const uint32_t *>(&v);
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t y;
@@ -379,7 +385,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
     if (!S::QREG) __syncthreads();
 
     // ---- the units of this warp: u0 + warp, + WARPS, ...
-    float M[NT][2], from[NT][2], l[NT][2], o[NT][HSEG * 4][4];  // (from: M, or 0 while that is -inf)
+    float M[NT][2], from[NT][2], l[NT][2], o[NT][HSEG * 4][4];  // (from: M less LIFT, or 0 while that is -inf)
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       M[t][0] = M[t][1] = -INFINITY;
@@ -441,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
               s[t][e] = __fmaf_rn((float)si[t][e], 65536.0f, __fmaf_rn((float)si[(NT + t) % S::CT][e], 256.0f, (float)si[(2 * NT + t) % S::CT][e]));
             }
           }
-        // ---- weights. A value scale below 2^-100 counts as 2^-100 (a block of zeros has scale 0): what it weighs
+        // ---- weights. A value scale below 2^-92 counts as 2^-92 (a block of zeros has scale 0): what it weighs
         // is below any other block's last place
         const float vs = !(vscale < LEAST) ? vscale : LEAST;
         const float lg = __log2f(vs), inv = __frcp_rn(vs);
@@ -483,7 +489,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
 #pragma unroll
               for (int x = 0; x < HSEG * 4; x++) o[t][x][p] *= by, o[t][x][2 + p] *= by;
               M[t][p] = m;
-              from[t][p] = m == -INFINITY ? 0.0f : m;
+              from[t][p] = m == -INFINITY ? 0.0f : m - LIFT;
             }
         }
         uint32_t ph[NT][2], pl[NT][2];
@@ -506,7 +512,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
             uint32_t hi = pack(w[2 * x], w[2 * x + 1]), lo = 0;
             if (!HALF) {
               const float2 b = unpack(hi);
-              lo = pack(w[2 * x] - b.x, w[2 * x + 1] - b.y);
+              lo = pack((w[2 * x] - b.x) * 2048.0f, (w[2 * x + 1] - b.y) * 2048.0f);
             }
             ph[t][x] = transposed(BOTH && c >= 2 ? lo : hi);
             if (PAIR) pl[t][x] = transposed(lo);
@@ -544,9 +550,14 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
             for (int t = 0; t < NT; t++) {
 #pragma unroll
               for (int y = 0; y < 2; y++) mma(o[t][m + y], a0[y], a1[y], a2[y], a3[y], ph[t][0], ph[t][1]);
-              if (PAIR) {
+            }
+            if (PAIR) {
+              // (the values go down by as much as the low parts went up, which is exact)
 #pragma unroll
-                for (int y = 0; y < 2; y++) mma(o[t][m + y], a0[y], a1[y], a2[y], a3[y], pl[t][0], pl[t][1]);
+              for (int y = 0; y < 2; y++) {
+                a0[y] = lowered(a0[y]), a1[y] = lowered(a1[y]), a2[y] = lowered(a2[y]), a3[y] = lowered(a3[y]);
+#pragma unroll
+                for (int t = 0; t < NT; t++) mma(o[t][m + y], a0[y], a1[y], a2[y], a3[y], pl[t][0], pl[t][1]);
               }
             }
           }
@@ -574,7 +585,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
 #pragma unroll
       for (int m = 0; m < HSEG * 4; m++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[0][m][e] += __shfl_xor_sync(0xffffffffu, o[0][m][e], 2);
+        for (int e = 0; e < 4; e++) o[0][m][e] += 4.8828125e-4f * __shfl_xor_sync(0xffffffffu, o[0][m][e], 2);  // 2^-11
     }
     __syncthreads();
     float *sums = reinterpret_cast<float *>(sm.ring);

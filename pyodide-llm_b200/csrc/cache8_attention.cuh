@@ -13,7 +13,10 @@ namespace cache8 {
 
 constexpr int UNIT = 16;             // positions of a unit, which lies within one block of the cache
 constexpr float RESCALE = 8.0f;      // log2 of how far a weight may rise above 1 before the running maximum moves
-constexpr float LEAST = 7.888609e-31f;  // 2^-100, see the weights' comment
+// Weights are 2^LIFT where a term is as large as the running maximum, so up to 2^15 before it moves: the upper end of
+// float16's range, whose lower end, 2^-24, is then 2^-31 of that term.
+constexpr float LIFT = 7.0f;
+constexpr float LEAST = 2.019484e-28f;  // 2^-92, see the weights' comment
 
 struct Args {
   void *out;

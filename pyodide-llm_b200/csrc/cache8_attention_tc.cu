@@ -194,9 +194,11 @@ __device__ __forceinline__ float hi_of(uint64_t v) { return __uint_as_float((uin
 
 // One step of this thread's row: 64 scores from tS, their weights over them. EDGE: some of the tile's rows don't see all
 // of the step; limit: the last position that this row sees, from the step's first. qf: what a score takes besides its key
-// scale, log2(e) / sqrt(hs) and the power of two that the row was divided by. m, l: the row's running maximum and sum. settle(by): called by the whole warp once m is settled, where some row's maximum moved with what the
-// row's sums go down by. (The next step's scores, loaded while this one's last weights are worked out, cost more than they saved: 189
-// us for 172, 102 for 97.)
+// scale, log2(e) / sqrt(hs) and the power of two that the row was divided by. m, l: the row's running maximum and sum.
+// The weights are relative to m, float32's to the step's own maximum (its products are added to the sums one step at a
+// time, so a step far below the others keeps its bits). settle(ref, by): called by the whole warp once that is known: ref,
+// and, float16, what the row's sums go down by where some row's m moved, else -1. (The next step's scores, loaded while
+// this one's last weights are worked out, cost more than they saved: 189 us for 172, 102 for 97.)
 template <int HP, bool HALF, bool EDGE, typename Settle>
 __device__ __forceinline__ void softmax_step(uint32_t tS, const float4 *sc, float qf, int limit, float &m, float &l,
                                              Settle &&settle) {
@@ -229,14 +231,24 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, const float4 *sc, floa
     top = fmaxf(top, x[u * UNIT + UNIT - 1]);
     most = fmaxf(most, __fmaf_rn(top, c[u], lg[u]));
   }
-  if (__any_sync(0xffffffffu, most > m + RESCALE)) {
-    const float top = fmaxf(m, most), by = m == top ? 1.0f : ex2(m - top);
-    l *= by, m = top;
-    settle(by);
+  float ref = most, step_by = 1.0f, step_l = 0.0f;
+  if (!HALF) {
+    const float top = fmaxf(m, most);
+    l *= m == top ? 1.0f : ex2(m - top);
+    step_by = most == top ? 1.0f : ex2(most - top);
+    m = top;
+    settle(most, -1.0f);
   } else {
-    settle(-1.0f);
+    if (__any_sync(0xffffffffu, most > m + RESCALE)) {
+      const float top = fmaxf(m, most), by = m == top ? 1.0f : ex2(m - top);
+      l *= by, m = top;
+      settle(m, by);
+    } else {
+      settle(m, -1.0f);
+    }
+    ref = m;
   }
-  const float from = m == -INFINITY ? 0.0f : m;
+  const float from = ref == -INFINITY ? 0.0f : ref - LIFT;
 #pragma unroll
   for (int u = 0; u < KU; u++) {
     const uint64_t c2 = f2(c[u], c[u]), a2 = f2(lg[u] - from, lg[u] - from);
@@ -253,10 +265,11 @@ __device__ __forceinline__ void softmax_step(uint32_t tS, const float4 *sc, floa
         lo[i / 2] = pack(w0 - b.x, w1 - b.y);
       }
     }
-    l = __fmaf_rn(lo_of(sum) + hi_of(sum), inv[u], l);
+    (HALF ? l : step_l) = __fmaf_rn(lo_of(sum) + hi_of(sum), inv[u], HALF ? l : step_l);
     st8(tS + 8 * u, hi);
     if (!HALF) st8(tS + 32 + 8 * u, lo);
   }
+  if (!HALF) l = __fmaf_rn(step_l, step_by, l);
   wait_st();
 }
 
@@ -690,10 +703,9 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
       ok = wait_for(&s.kv_full[j % STAGES], (j / STAGES) & 1, error, 117) && ok;
       ok = __all_sync(0xffffffffu, ok);
       fence_after();
-      // where a row's maximum moves, to m, and its sums go down by `by`; by < 0: nowhere in the warp
-      auto settle = [&](float by) {
+      auto settle = [&](float ref, float by) {
         if (!HALF) {
-          s.ref[j & 7][y] = m;
+          s.ref[j & 7][y] = ref;
           __syncwarp();
           if (lane == 0) mbar_arrive(&s.ref_full[j & 7]);
         } else if (by >= 0.0f && j > 0) {  // (whole warps come here: TMEM is read and written by whole warps)

@@ -110,3 +110,87 @@ def test_attention_check_reads_the_scratch():
     assert "104" in abi.last_error()
     c.call()
     assert lib.b200k_cache8_attention_check(ptr(c.scratch), None) == 0
+
+
+# ------------------------------------------------------------------------------------------------------- precision
+
+def exact(c):
+    """(out, bound) of a case in float64. bound: what the header allows, by its terms, u = 2^-24 half a step of float32:
+    - a query value is off by 2^-22 of itself (two float16 parts) or 2^-30 of its row's largest (digits of a byte);
+    - a score's products, added in float32: (size / 8 + 4) times 4 u of the sum of their sizes (the tensor cores cut off);
+    - the exponent: half a step of the score, the value scale's logarithm and the maximum each, twice, and 2^x;
+    - sums over the positions: by steps of 64, 2 u each of the whole, and 64 u for joining the parts;
+    - a weight in two float16 parts: 2^-22 of itself, and half a step, 2^-32, of the largest of its 64 positions (times value
+      scale). Float16: half a step, 2^-11, and no finer than 2^-32 of the row's largest; the output half a step."""
+    u = 2.0 ** -24
+    size, group = c.hs, c.heads // c.nkv
+    out, bound = np.zeros(c.q64.shape), np.zeros(c.q64.shape)
+    for i, length in enumerate(c.lengths):
+        rows, page = int(c.news[i]), c.tables[i, :-(-c.lengths[i] // c.block)].astype(int)
+        for h in range(c.heads):
+            kv = h // group
+            k = (c.kc[page, kv].astype(np.float64) * c.ks[page, kv].astype(np.float64)[:, None, None]).reshape(-1, size)
+            v_int = np.abs(c.vc[page, kv].astype(np.float64)).reshape(-1, size)
+            vs = np.repeat(c.vs[page, kv].astype(np.float64), c.block)
+            v = c.vc[page, kv].reshape(-1, size) * vs[:, None]
+            for j in range(rows):
+                t, seen = c.starts[i] + j, int(length) - rows + j + 1
+                q = c.q64[t, h]
+                s = k[:seen] @ q / np.sqrt(size)
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                out[t, h] = p @ v[:seen]
+                off = np.abs(k[:seen]) @ (np.abs(q) * 2.0 ** -22 + np.abs(q).max() * 2.0 ** -30)
+                off += np.abs(k[:seen]) @ np.abs(q) * (size / 8 + 4) * 4 * u
+                largest = np.abs(s).max() * 1.4427 + np.abs(np.log2(vs[:seen])).max()
+                weight = (off / np.sqrt(size)).max() + (4 * largest + 64) * u + 2.0 ** -22
+                whole = p @ np.abs(v[:seen])
+                bound[t, h] = whole * (2 * weight + (2 * (seen // 64 + 1) + 64) * u)
+                pv = p * vs[:seen]
+                for at in range(0, seen, 64):
+                    few = slice(at, min(seen, at + 64))
+                    bound[t, h] += 2.0 ** -32 * (pv.max() if c.half else pv[few].max()) * v_int[few].sum(0)
+                if c.half:
+                    bound[t, h] += whole * 2.0 ** -11 + np.abs(out[t, h]) * 2.0 ** -11 + 2.0 ** -25
+    return out, bound
+
+
+def check_exact(c):
+    got = c.run()
+    want, bound = exact(c)
+    off = np.abs(got - want)
+    assert (off <= bound).all(), (np.argwhere(~(off <= bound))[:5], np.nanmax(off / bound), np.nanmax(off))
+    return got
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("below", [9.0, 17.0, 22.0])
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("requests,heads", [([(8192, 70)], 1), ([(20000, 1)] * 24, 1), ([(20000, 1)] * 12, 8)])
+def test_attention_of_weights_far_below_the_largest(requests, heads, hs, below, half):
+    """One position (of values 0) far above a flat rest, whose weights are what the output consists of."""
+    c = Case(requests, heads, 1, hs, 64, half, seed=3)
+    c.q[:] = 1
+    c.kc[:], c.ks[:], c.vs[:] = 0, below / (127 * np.sqrt(hs)), 0.03
+    c.vc[:] = np.abs(c.vc)
+    for i in range(len(requests)):
+        c.kc[c.tables[i, 0], :, 0] = 127
+        c.vc[c.tables[i, 0], :, 0] = 0
+    check_exact(c)
+
+
+# ---------------------------------------------------------------------------------------------------- long prompts
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("hs", [64, 128])
+def test_prompts_of_many_steps(hs, half):
+    """Prompts of 25 and more steps of 64 positions, past the length of every ring of the prompt kernel: float32's maxima on
+    their way from the softmax to the sums (8), scores (2 to 4), keys and values (4). Keys that grow along the first
+    request, so that a row's maximum moves all the way; the same bits again."""
+    c = Case([(1700, 1100), (1600, 1600), (2500, 70)], 2, 1, hs, 32, half, seed=hs)
+    for j, b in enumerate(c.tables[0, :-(-1700 // 32)]):
+        c.ks[b] = 0.0005 * (j + 1)
+    got = check_exact(c)
+    for _ in range(3):
+        c.call()
+        assert np.array_equal(c.result(), got)
