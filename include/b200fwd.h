@@ -342,10 +342,11 @@ int b200k_cache8_load(void *k, void *v, const int8_t *kc, const float *ks, const
  * sees no position (fewer positions than tokens) is 0; a row that sees a position whose table entry is no block, or
  * past its table row, is NaN. Rows that belong to no request are left as they were; starts that do not ascend within
  * 0..n leave out unwritten. Not to the bit like b200k_attention, but within float32's rounding of the exact result for
- * the stored values, with these limits (a weight: softmax's times the value scale): a float32 row's weights count in 22
- * bits, and among 64 positions in steps of 2^-31 of their largest at the finest; a float16 row's in 11 bits, in steps of
- * 2^-31 of the row's largest; value scales below 2^-92 count as that. The same call gives the same bits. Up to 65536
- * requests, n up to 2^25 and n * nh to 2^30, table_width * block up to 2^30. scratch: b200k_cache8_attention_scratch() bytes of device memory, 256-byte aligned,
+ * the stored values, with these limits (a weight: softmax's times the value scale): a query value counts in 22 bits, or
+ * in steps of 2^-29 of its row's largest; a float32 row's weights count in 22 bits, and among 64 positions in steps of
+ * 2^-31 of their largest at the finest; a float16 row's in 11 bits, in steps of 2^-31 of the row's largest; value scales
+ * below 2^-92 count as that. The same call gives the same bits. Up to 65536 requests, n up to 2^25 and n * nh to 2^30,
+ * table_width * block up to 2^30. scratch: b200k_cache8_attention_scratch() bytes of device memory, 256-byte aligned,
  * nothing zeroed; calls that overlap on the GPU need one each. */
 int b200k_cache8_attention(void *out, const void *q, const int8_t *kc, const float *ks, const int8_t *vc,
                            const float *vs, const int32_t *tables, const int32_t *starts, const int32_t *lengths,

@@ -7,8 +7,9 @@
 // operand; the scales stay outside (a block's key scale on its scores, its value scale within its weights), so the
 // cache's values are never rounded.
 //  - scores: the keys' bytes as they are (m16n8k32, signed bytes, exact int32 sums) with the queries in fixed point, each
-//    row by a power of two into (0, 2) and then as three digits of a byte, 21 bits behind the point: a column for each
-//    digit of each row, whose sums are put together in float32.
+//    row by a power of two into (0, 2) and then as four digits of a byte, 29 bits behind the point (a value is off by
+//    2^-30 of its row's largest at most; with three digits an outlier of 1000 cost the others all below 2^-12 of their
+//    size): a column for each digit of each row, whose sums are put together in float32.
 //  - values: as float16 integers (exact), with the weights as a float16 pair high + low / 2^11, the low part taken so far up
 //    that it keeps its 11 bits down to 2^-43 of the largest weight (float16 queries: one float16, half a step of the
 //    output's type, down to 2^-31 of the largest).
@@ -147,7 +148,7 @@ struct Shape {
   static constexpr bool BOTH = RT == 4;
   static constexpr int NT = BOTH ? 1 : RT / 8;      // row tiles of the value products
   // the score products: 32 values of the head an instruction, columns by digit, then row
-  static constexpr int KSTEPS = HSEG * 2, CT = (3 * RT + 7) / 8;
+  static constexpr int KSTEPS = HSEG * 2, CT = RT / 2;
   static constexpr int VB = HSEG % 2 ? 8 : 16;      // bytes of a lane's piece of a value row
   static constexpr int VN = HP / (8 * VB);          // pieces
   static constexpr int ROW = HSEG <= 2 ? HP : 256;  // bytes of a row in the ring
@@ -333,9 +334,11 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
           }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = min(max((int)(top >> 23) - 127, -126), 126);
-        f[t] = __uint_as_float((uint32_t)(127 - e) << 23);
-        back[t] = __uint_as_float((uint32_t)(127 + e) << 23) * 4.76837158203125e-7f;  // 2^-21
+        // (rows below 2^-90 as if they were of that size: what they are scaled back by stays a whole float32; 2^-127, for
+        // the largest, is a subnormal)
+        const int e = min(max((int)(top >> 23) - 127, -90), 127);
+        f[t] = __uint_as_float(max((uint32_t)(127 - e) << 23, 0x400000u));
+        back[t] = __uint_as_float((uint32_t)(127 + e) << 23) * 1.862645149230957e-9f;  // 2^-29
         if (top >= 0x7f800000u) back[t] = __uint_as_float(0x7fffffffu);  // (a row with an infinity or a NaN: NaN)
         qf[t][0] = __shfl_sync(0xffffffffu, back[t], BOTH ? 8 * (c & 1) : 8 * c) * a.scale;
         qf[t][1] = __shfl_sync(0xffffffffu, back[t], BOTH ? 8 * (c & 1) + 4 : 8 * c + 4) * a.scale;
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
       for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int i = 0; i < S::KSTEPS; i++) {
-          uint32_t word[3][2] = {};
+          uint32_t word[4][2] = {};
           const int d = 64 * (i / 2) + 16 * c + 8 * (i & 1);
           if (is[t] && (WHOLE || d < hs)) {
 #pragma unroll
@@ -357,20 +360,20 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
               query<HALF>(a.q, off[t] + d + 4 * y, z);
 #pragma unroll
               for (int e = 0; e < 4; e++) {
-                // q 2^21 = 65536 d0 + 256 d1 + d2, the digits from -128 to 127: with 128 added to the lower two, the
-                // bytes of the sum, less that
-                const uint32_t sum = (uint32_t)(__float2int_rn(z[e] * f[t] * 2097152.0f) + 0x8080) ^ 0x8080u;
+                // q 2^29 = 2^24 d0 + 2^16 d1 + 2^8 d2 + d3, the digits from -128 to 127: with 128 added to the lower
+                // three, the bytes of the sum, less that
+                const uint32_t sum = (uint32_t)(__float2int_rn(z[e] * f[t] * 536870912.0f) + 0x808080) ^ 0x808080u;
 #pragma unroll
-                for (int k = 0; k < 3; k++) word[k][y] |= (sum >> (16 - 8 * k) & 255) << (8 * e);
+                for (int k = 0; k < 4; k++) word[k][y] |= (sum >> (24 - 8 * k) & 255) << (8 * e);
               }
             }
           }
           if (BOTH) {
             keep(i * S::CT, g < 4 ? word[0][0] : word[1][0], g < 4 ? word[0][1] : word[1][1]);
-            keep(i * S::CT + S::CT - 1, g < 4 ? word[2][0] : 0, g < 4 ? word[2][1] : 0);
+            keep(i * S::CT + 1, g < 4 ? word[2][0] : word[3][0], g < 4 ? word[2][1] : word[3][1]);
           } else {
 #pragma unroll
-            for (int k = 0; k < 3; k++) keep((i * S::CT + k * NT + t) % (S::KSTEPS * S::CT), word[k][0], word[k][1]);
+            for (int k = 0; k < 4; k++) keep((i * S::CT + k * NT + t) % (S::KSTEPS * S::CT), word[k][0], word[k][1]);
           }
         }
     }
@@ -440,11 +443,13 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             if (BOTH) {
-              // lanes c < 2 have the first digits and the last ones, c >= 2 the second ones, of the same rows
-              const float v = (float)si[0][e] * (c < 2 ? 65536.0f : 256.0f) + (float)si[S::CT - 1][e];
+              // lanes c < 2 have the first and the third digits, c >= 2 the second and the last ones, of the same rows
+              const float v = (float)si[0][e] * (c < 2 ? 16777216.0f : 65536.0f) + (float)si[1][e] * (c < 2 ? 256.0f : 1.0f);
               s[t][e] = v + __shfl_xor_sync(0xffffffffu, v, 2);
             } else {
-              s[t][e] = __fmaf_rn((float)si[t][e], 65536.0f, __fmaf_rn((float)si[(NT + t) % S::CT][e], 256.0f, (float)si[(2 * NT + t) % S::CT][e]));
+              s[t][e] = __fmaf_rn((float)si[(2 * NT + t) % S::CT][e], 256.0f, (float)si[(3 * NT + t) % S::CT][e]);
+              s[t][e] = __fmaf_rn((float)si[(NT + t) % S::CT][e], 65536.0f, s[t][e]);
+              s[t][e] = __fmaf_rn((float)si[t][e], 16777216.0f, s[t][e]);
             }
           }
         // ---- weights. A value scale below 2^-92 counts as 2^-92 (a block of zeros has scale 0): what it weighs

@@ -632,8 +632,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     if (HALF) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     else if (SOFT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
-    // ---- the softmax of tile t_own. Its queries first, as float16 (float32: by a power of two into (0, 2), in two parts)
-    // in the swizzled layout
+    // ---- the softmax of tile t_own. Its queries first, as float16 (float32: in two parts, by a power of two to below 2^15,
+    // so that the low part, which ends at 2^-24, reaches down to 2^-39 of the row's largest) in the swizzled layout
     const int t = t_own, soft = SOFT == 2 ? (warp - BRINGERS / 32) >> 2 : 0;
     float qf = a.scale;
     s.row[t][y] = make_int2(on ? r.first + token : -1, head);  // (SOFT 2: both warpgroups write, the same)
@@ -667,7 +667,8 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
             for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(z[k]));
 #pragma unroll
             for (int d = LANES / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -126), 126);
+            // (rows below 2^-112 as if they were of that size: the powers have to be whole float32)
+            const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -112), 127) - 14;
             const float f = __uint_as_float((uint32_t)(127 - e) << 23);
             if (col == 0) s.power[row] = __uint_as_float((uint32_t)(127 + e) << 23);
             uint32_t p[4], q[4];

@@ -194,3 +194,18 @@ def test_prompts_of_many_steps(hs, half):
     for _ in range(3):
         c.call()
         assert np.array_equal(c.result(), got)
+
+
+# four, eight and sixteen rows a tile, and prompts
+KINDS = [([(300, 1), (200, 1)], 4, 2), ([(300, 1), (200, 1)], 8, 2), ([(300, 3), (77, 2)], 8, 1), (PROMPTS, 2, 1)]
+
+
+@pytest.mark.parametrize("half,outlier", [(False, 30), (False, 1000), (False, 1e5), (True, 30), (True, 1e4)])
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("requests,heads,nkv", KINDS)
+def test_attention_of_queries_with_an_outlier(requests, heads, nkv, hs, half, outlier):
+    """A query value far above the others, where the keys are 0: the others' scores stay."""
+    c = Case(requests, heads, nkv, hs, 16, half, seed=hs)
+    c.q.reshape(c.n, heads, hs)[:, :, 5] = outlier
+    c.kc[..., 5] = 0
+    check_exact(c)
