@@ -328,6 +328,20 @@ __device__ __forceinline__ void values_of(const uint4 &u, float (&x)[8]) {
   }
 }
 
+// What kernels before this one in the stream may write while this one is already there (its wait is at its beginning), so
+// no loads for memory that stays as it is; volatile, so none comes before that wait, and not held back by the stores
+// between them, which go elsewhere.
+__device__ __forceinline__ uint4 vector_at(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ int slot_at(const int32_t *p) {
+  int v;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+
 // the integer nearest to q a / b, half to even, in 64 bits: q a is exact there (q an integer of 8 bits, or 1 and a a
 // float), and so far from a half that is not one that the quotient's rounding cannot reach it. At most 127 in size: a
 // scale of a few of float32's smallest steps may be a third below the largest value's 127th part (and has no inverse, so
@@ -416,11 +430,11 @@ __global__ void __launch_bounds__(ST, 8) cache8_store_kernel(StoreArgs a) {
                   ((int64_t)h * a.hs + col) * (HALF ? 2 : 4);
   // a single token's vector, on its way before its slot is known
   uint4 first = make_uint4(0, 0, 0, 0);
-  if (TEAM < ST && row == 0) first = __ldg(reinterpret_cast<const uint4 *>(x));
+  if (TEAM < ST && row == 0) first = vector_at(x);
   const uint32_t inverse = inverse_of(a.block);
   // the block of token i, or -1 (a lane a token, every warp by itself)
   auto page_of = [&](int i) {
-    const int slot = i >= 0 && i < a.n ? __ldg(a.slots + i) : -1;
+    const int slot = i >= 0 && i < a.n ? slot_at(a.slots + i) : -1;
     const int page = slot < 0 ? -1 : over(slot, a.block, inverse);
     return page < a.blocks ? page : -1;
   };
@@ -432,7 +446,7 @@ __global__ void __launch_bounds__(ST, 8) cache8_store_kernel(StoreArgs a) {
   int turn = 0;
   for (; begins; begins &= begins - 1) {
     const int k = __ffs(begins) - 1, i = i0 + k, page = __shfl_sync(0xffffffffu, mine, k);
-    const int slot = __ldg(a.slots + i), held = slot - page * a.block;  // held: earlier tokens in the block
+    const int slot = slot_at(a.slots + i), held = slot - page * a.block;  // held: earlier tokens in the block
     float *scale = scales + (int64_t)page * a.nkv + h;
     const float s_old = held ? *scale : 0.0f;
     const uint32_t end = ends >> k;
@@ -450,7 +464,7 @@ __global__ void __launch_bounds__(ST, 8) cache8_store_kernel(StoreArgs a) {
     const char *src = x + k * step;
     auto vector = [&](int u) {
       const int r = row + u * rows, t = parts == 2 ? r >> 1 : r;
-      return __ldg(reinterpret_cast<const uint4 *>(src + t * step + (parts == 2 ? (r & 1) * vpr * 16 : 0)));
+      return vector_at(src + t * step + (parts == 2 ? (r & 1) * vpr * 16 : 0));
     };
     uint4 kept[KEEP];
     float top = 0.0f;
@@ -500,7 +514,7 @@ __global__ void __launch_bounds__(ST, 8) cache8_store_kernel(StoreArgs a) {
       const int r = row + u * rows, t = parts == 2 ? r >> 1 : r;
       float y[VW];
       values_of(v, y);
-      int8_t *q = dst + (__ldg(slots + t) - base) * a.hs + (parts == 2 ? (r & 1) * vpr * VW : 0);
+      int8_t *q = dst + (slot_at(slots + t) - base) * a.hs + (parts == 2 ? (r & 1) * vpr * VW : 0);
       if (HALF)
         *reinterpret_cast<uint2 *>(q) = some ? make_uint2(four_bytes(y, s, inv), four_bytes(y + VW - 4, s, inv)) : make_uint2(0, 0);
       else *reinterpret_cast<uint32_t *>(q) = some ? four_bytes(y, s, inv) : 0;

@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(THREADS, 1) cache8_attention_tc_kernel(const A
     auto load = [&](uint4 &k, uint4 &v, int page, int at) {
       if ((uint32_t)page < (uint32_t)a.blocks && in_head) {
         const int64_t off = (int64_t)page * page_bytes + (head_bytes + at * a.hs);
-        k = __ldg(reinterpret_cast<const uint4 *>(a.kc + off)), v = __ldg(reinterpret_cast<const uint4 *>(a.vc + off));
+        k = *reinterpret_cast<const uint4 *>(a.kc + off), v = *reinterpret_cast<const uint4 *>(a.vc + off);
       }
     };
     auto widened = [&](uint8_t *tile, int i, const uint4 &v) {
