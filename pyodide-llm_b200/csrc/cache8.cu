@@ -492,6 +492,7 @@ __global__ void __launch_bounds__(ST, 8) cache8_store_kernel(StoreArgs a) {
     if (!(s_old <= s)) s = s != s ? s : s_old;
     const float inv = s > 1e-37f ? __fdiv_rn(1.0f, s) : 0.0f;
     int8_t *dst = cache + ((int64_t)page * a.nkv + h) * a.block * a.hs;
+    if (TEAM < ST) __syncwarp();  // (every lane has read the scale)
     if (tid == 0) *scale = s;
     if (s > s_old && s_old > 0) {
       // the earlier tokens' integers to the new step
