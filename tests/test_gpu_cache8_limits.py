@@ -209,3 +209,13 @@ def test_attention_of_queries_with_an_outlier(requests, heads, nkv, hs, half, ou
     c.q.reshape(c.n, heads, hs)[:, :, 5] = outlier
     c.kc[..., 5] = 0
     check_exact(c)
+
+
+@pytest.mark.parametrize("requests,heads,nkv", KINDS)
+def test_attention_of_the_largest_queries(requests, heads, nkv):
+    """float32 queries up to the type's largest, over keys so small that the scores are ordinary."""
+    c = Case(requests, heads, nkv, 64, 16, False, seed=9)
+    c.q[:] = np.sign(c.q) * np.finfo(np.float32).max * np.random.default_rng(9).uniform(0.1, 1, c.q.shape)
+    c.q[:, ::7] = np.finfo(np.float32).max * np.sign(c.q[:, ::7])
+    c.ks[:] = 2.0 ** -133
+    check_exact(c)
