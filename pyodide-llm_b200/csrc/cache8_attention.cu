@@ -755,21 +755,25 @@ int rows_of_tile(int n, int n_seqs, int group, bool half) {
   return !half && rows <= 4 * (int64_t)n_seqs ? 4 : rows <= 8 * (int64_t)n_seqs ? 8 : 16;
 }
 
+// The scratch: as much as any tile height of up to 16 takes, so that it never shrinks as n or n_seqs grow (rows_of_tile goes
+// up with one and down with the other), and a scratch for the most of both serves every call of no more.
 struct Layout {
   int rt;
-  int64_t tiles, parts;
+  int64_t tiles;
   uint64_t ml_at, part_at, bytes;
 };
 Layout layout_of(int n, int n_seqs, int nh, int nkv, int hs, bool half) {
   Layout s;
   const int group = nh / nkv;
   s.rt = rows_of_tile(n, n_seqs, group, half);
-  s.tiles = ((int64_t)n * group + s.rt - 1) / s.rt + (n < n_seqs ? n : n_seqs);
-  s.parts = s.tiles + (MOST_BLOCKS + nkv - 1) / nkv;
+  const int64_t rows = (int64_t)n * group, requests = n < n_seqs ? n : n_seqs;
+  s.tiles = (rows + s.rt - 1) / s.rt + requests;
+  // rows of partial sums: those of (tiles + spans) tiles, of 4 rows as of 16
+  const uint64_t parts = (rows + 16 * (1 + requests + (MOST_BLOCKS + nkv - 1) / nkv)) * nkv;
   const auto up = [](uint64_t x) { return (x + 255) / 256 * 256; };
-  s.ml_at = up((s.tiles + 1) * sizeof(int4));
-  s.part_at = s.ml_at + up(s.parts * nkv * s.rt * sizeof(float2));
-  s.bytes = s.part_at + up(s.parts * nkv * s.rt * (uint64_t)hs * sizeof(float));
+  s.ml_at = up(((rows + 3) / 4 + requests + 1) * sizeof(int4));
+  s.part_at = s.ml_at + up(parts * sizeof(float2));
+  s.bytes = s.part_at + up(parts * (uint64_t)hs * sizeof(float));
   return s;
 }
 

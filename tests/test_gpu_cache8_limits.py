@@ -1,11 +1,14 @@
 """Where the paged 8-bit cache and its attention can go wrong: queries and keys of zeros, queries of any size, scales at
 float32's lower end, starts that do not ascend, outliers among a query's values, weights far below the largest one, and
 requests of more steps than the prompt kernel's rings hold. GPU only."""
+import ctypes
+
 import numpy as np
 import pytest
+import torch
 
 from b200fwd import abi
-from gpu_util import host, ptr
+from gpu_util import full, host, ptr
 from test_gpu_cache8 import Case, store_case
 
 pytestmark = pytest.mark.gpu
@@ -219,3 +222,17 @@ def test_attention_of_the_largest_queries(requests, heads, nkv):
     c.q[:, ::7] = np.finfo(np.float32).max * np.sign(c.q[:, ::7])
     c.ks[:] = 2.0 ** -133
     check_exact(c)
+
+
+def test_attention_in_the_scratch_of_a_larger_call():
+    """Fewer requests and tokens, but taller tiles, in a scratch sized for more of both: nothing behind it is touched."""
+    lib, size = abi.load(), ctypes.c_uint64()
+    c = Case([(3000, 3), (700, 2)], 8, 1, 64, 16, False, seed=2)
+    c.upload()
+    c.dq_wide = torch.cat([c.dq, c.dq[:1].expand(c.behind, -1)]).contiguous()
+    abi.check(lib.b200k_cache8_attention_scratch(c.n + c.behind, 64, 8, 1, 64, 0, ctypes.byref(size)))
+    room = int(size.value) // 4
+    c.scratch = full(room + (1 << 20), -77, np.int32)
+    c.call()
+    c.check(c.result())
+    assert (host(c.scratch)[room:] == -77).all()
