@@ -236,3 +236,19 @@ def test_attention_in_the_scratch_of_a_larger_call():
     c.call()
     c.check(c.result())
     assert (host(c.scratch)[room:] == -77).all()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("hs", [16, 32, 80, 96])
+def test_prompts_of_padded_heads(hs, half):
+    """Head sizes that the prompt kernel pads to 64 or 128."""
+    c = Case(PROMPTS, 3, 1, hs, 48, half, seed=hs)
+    check_exact(c)
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_attention_of_single_tokens_in_wide_buffers(half):
+    """A step of single tokens in buffers of 1000 rows, as a captured step makes it: the rows behind them stay."""
+    c = Case([(300 + 17 * i, 1) for i in range(20)], 8, 2, 128, 32, half, seed=1)
+    c.behind = 980
+    check_exact(c)
