@@ -363,7 +363,7 @@ int b200k_cache8_attention_check(const void *scratch, b200fwd_stream stream);
  * in nats (NULL: not wanted), and the k (0 to 32) most probable ids with their log probabilities, top_id and top_logprob
  * [count][k], the largest first, ties by the lowest id. Masked logits may be -inf (log probability -inf) or any lowest
  * value. A row without a finite largest logit (all -inf, or an infinity or a NaN in it) gives NaN and ids -1. Float32
- * arithmetic whatever the logits; no scratch. */
+ * arithmetic whatever the logits (a row of 2^30: off by 1e-4); no scratch. */
 int b200k_logprobs(float *logprob, float *entropy, float *top_logprob, int32_t *top_id, const void *logits,
                    const int32_t *targets, int32_t count, int32_t n, int64_t stride, int32_t k, int32_t half,
                    b200fwd_stream stream);

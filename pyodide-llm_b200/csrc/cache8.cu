@@ -656,7 +656,9 @@ extern "C" int b200k_block_tables(int32_t *tables, int32_t *ring, int32_t *state
       return fail(B200FWD_EINVAL, "block_tables: 1 block at least, and positions and slots that an int32 holds");
     TablesArgs a = {tables, ring, state_out, lengths_out, starts, slots, seq, pos, state, lengths, news,
                     n_seqs, table_width, blocks, block, n, n > ROWS_APART};
-    // one block up to 4096 tokens and 2 tiles of requests, else a cluster of eight
+    // One block up to 4096 tokens and 2 tiles of requests, else a cluster of eight. Measured, one and eight: 64 requests of a
+    // token each 5.4 and 6.2 us, 64 of 64 tokens 8.0 and 6.3, 1000 of one 12.7 and 13.1, 1025 of three 15.0 and 14.9, 1000
+    // of 64 16.4 and 14.3.
     const unsigned ranks = n <= 4096 && n_seqs <= 2 * TT ? 1 : 8;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -697,7 +699,10 @@ extern "C" int b200k_cache8_store(int8_t *kc, float *ks, int8_t *vc, float *vs, 
     if (rc) return rc;
     StoreArgs a = {{kc, vc}, {ks, vs}, {k, v}, {k_stride, v_stride}, slots, n, blocks, block, nkv, hs, 0};
     // Up to 512 tokens a warp each (and head), so that single ones are stored side by side; else a thread block for the runs
-    // that begin among 16, which are few where prompts are stored.
+    // that begin among 16, which are few where prompts are stored. What tells the two apart is the runs' length, which only
+    // the device knows; n stands for it. Measured (8 heads of 128, float32 and float16, by warps and by blocks): 64 single
+    // tokens 3.3 and 4.9 us, 19 and 24; 512 of them 7.2 and 8.6, 27 and 30; 1024 12 and 14, 31 and 33. One prompt of 512
+    // tokens 15 and 34, 6.7 and 6.6; of 1024 20 and 38, 8 and 12; 64 of 73 tokens 42 and 56, 20 and 23.
     if (n <= 512) {
       a.per = 1;
       launch(half ? cache8_store_kernel<true, 32> : cache8_store_kernel<false, 32>, dim3(n, (2 * nkv + 3) / 4), dim3(ST), 0,

@@ -69,7 +69,10 @@ __device__ __forceinline__ uint32_t widen(uint32_t biased) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// cache8_attention_tc.cu: the requests of more than ROWS_FEW rows of a kv head
+// cache8_attention_tc.cu: the requests of more than ROWS_FEW rows of a kv head. Measured with 8 requests of 2000 positions, 8
+// kv heads, here and there: float32 with heads of 64, 16 rows 36 and 37 us, 32 38 and 37, 64 49 and 37, 128 80 and 37;
+// with heads of 128, 32 rows 48 and 59, 64 65 and 60, 128 107 and 61; float16 with heads of 128, 32 rows 44 and 42, 64 57
+// and 42, 128 92 and 42.
 constexpr int ROWS_FEW = 64;
 int launch_attention8_prompts(const Args &a, bool half, cudaStream_t stream);
 // head sizes that it takes

@@ -22,8 +22,8 @@
 // issue slots 1400; a block begins and ends in 15,000 (the queries, the first keys, the first scores; rows out) beside 30
 // steps on average. Float32, heads of 64: 1550 a step of one tile (one warpgroup of softmax: 2060), of which the products
 // are about 900; each softmax step takes 2300 to 2600, twice its instructions' issue slots.
-// Measured: 8 requests that add 260 to 509 tokens to contexts of up to 4500, 32 query and 8 kv heads of 128, float16: 172 us
-// (0.64 PFLOP/s of what the masks leave); 4 whole prompts of 2048 tokens, 8 heads of 64, float32: 87 us.
+// Measured: 8 requests that add 260 to 509 tokens to contexts of up to 4500, 32 query and 8 kv heads of 128, float16: 168 us
+// (0.66 PFLOP/s of what the masks leave); 4 whole prompts of 2048 tokens, 8 heads of 64, float32: 87 us.
 // TMEM (512 columns), float16: tile t's two score buffers at 128 t + {0, 64}, its O at 256 + t * head size; float32: three
 // score buffers (heads of up to 64: four) at 64 u, two of O behind them.
 // Every wait is bounded: past it the kernel sets the scratch's error word (b200k_cache8_attention_check) and runs to its end.
@@ -39,7 +39,10 @@ namespace {
 using namespace tc;
 
 constexpr int QT = 128, KT = 64, THREADS = 640, KU = KT / UNIT;
-constexpr int SORTED = 64;     // requests that are taken in order of their lengths
+// Requests that are taken in order of their lengths. Measured, sorted and not (prompt blocks over up to 4000 positions, 32 query
+// and 8 kv heads of 128, float16): 8 requests 121 and 127 us, 64 176 and 216; 65, with a limit of 512, 181 and 217, 128 362
+// and 385.
+constexpr int SORTED = 64;
 
 template <int HP, bool HALF>
 struct Tc {

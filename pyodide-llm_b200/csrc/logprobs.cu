@@ -14,7 +14,7 @@
 // A row's partial results meet in one block of its cluster, a different one from row to row, which adds them in the
 // blocks' order while the others go on (the cluster's barrier is waited for a row later).
 // Measured at 128256 float32 logits: 512 rows 53 us without alternatives (4.9 TB/s, 0.75 of a copy's rate), 63 us with
-// 20; 64 rows 12 and 17 us, of which a row's chain of exchanges is most. One row of 1024: 3.6 and 6.2 us.
+// 20; 64 rows 11 and 16 us, of which a row's chain of exchanges is most. One row of 1024: 3.6 and 6.2 us.
 #include <cuda_fp16.h>
 
 #include <atomic>
@@ -572,7 +572,9 @@ int launch_logprobs(const Args &a, int count, cudaStream_t stream) {
   auto kernel = logprobs_kernel<HALF>;
   constexpr int smem = GROUPS * GROUP * T * 16;
   // Blocks of a row: one where the rows fill the GPU (a block's work on a row beyond its values is then done once), more
-  // while the GPU has room for all rows' blocks and a thread more than one vector.
+  // while the GPU has room for all rows' blocks and a thread more than one vector. Measured (128256 float32 logits, k 5): a
+  // row by one block 18.1 us, by eight 9.8; 64 rows by one 19.4, by four 14.1, by eight 21.3; 148 by one 19.5, by two 18.7,
+  // by four 31.3. (37 rows by eight take 19.5, by one 18.8: 32 clusters of eight are resident at once.)
   const int vecs = (a.n + VW - 1) / VW;
   int ranks = 1;
   while (ranks < 8 && count * ranks * 2 <= 148 * RESIDENT && vecs > ranks * T) ranks *= 2;
