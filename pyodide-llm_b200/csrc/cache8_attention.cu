@@ -879,9 +879,10 @@ extern "C" int b200k_cache8_attention(void *out, const void *q, const int8_t *kc
     // blocks of tokens go to the tensor cores; where there is no more than a token a request on average (of the buffers'
     // rows), any request is taken here, and one kernel less launched
     const bool prompts = n > n_seqs && prompts_fit(hs);
-    // Tables of no more positions than a span has: a thread block a tile, and nothing to join. Measured, so and by spans: 3
-    // requests of 333 positions 8.7 and 16.7 us, 64 of 512 23.7 and 28; 256 of 300 66 and 61.
-    const bool whole_tiles = (int64_t)table_width * block <= MIN_UNITS * UNIT;
+    // Tables of no more positions than a span has: a thread block a tile, and nothing to join. No more requests than a block
+    // looks over at once, as every block does (65,536 of them take 66 ms so). Measured, so and by spans: 3 requests of 333
+    // positions 8.7 and 16.7 us, 64 of 512 23.7 and 28; 256 of 300 66 and 61.
+    const bool whole_tiles = (int64_t)table_width * block <= MIN_UNITS * UNIT && n_seqs <= THREADS;
     Args a = {out, q, kc, vc, ks, vs, tables, starts, lengths, reinterpret_cast<int4 *>(base) + 1,
               reinterpret_cast<float2 *>(base + s.ml_at), reinterpret_cast<float *>(base + s.part_at), q_stride,
               out_stride, n, n_seqs, table_width, blocks, block, nkv, hs, nh / nkv,

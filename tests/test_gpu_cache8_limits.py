@@ -252,3 +252,11 @@ def test_attention_of_single_tokens_in_wide_buffers(half):
     c = Case([(300 + 17 * i, 1) for i in range(20)], 8, 2, 128, 32, half, seed=1)
     c.behind = 980
     check_exact(c)
+
+
+@pytest.mark.parametrize("requests", [128, 129, 1000])
+def test_attention_of_many_short_requests(requests):
+    """Short tables of as many requests as one look takes, of one more, and of many."""
+    rng = np.random.default_rng(requests)
+    c = Case([(int(rng.integers(1, 80)), int(rng.integers(0, 2))) for _ in range(requests)], 4, 2, 32, 16, False, seed=requests)
+    check_exact(c)
