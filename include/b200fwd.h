@@ -347,7 +347,8 @@ int b200k_cache8_load(void *k, void *v, const int8_t *kc, const float *ks, const
  * 2^-31 of their largest at the finest; a float16 row's in 11 bits, in steps of 2^-31 of the row's largest; value scales
  * below 2^-92 count as that. The same call gives the same bits. Up to 65536 requests, n up to 2^25 and n * nh to 2^30,
  * table_width * block up to 2^30. scratch: b200k_cache8_attention_scratch() bytes of device memory, 256-byte aligned,
- * nothing zeroed, for this n and n_seqs or larger ones; calls that overlap on the GPU need one each. */
+ * nothing zeroed, for this n and n_seqs or larger ones; calls that overlap on the GPU need one each. (n, the buffers' rows,
+ * also chooses the kernels: where no request adds more than a token, an n of no more than n_seqs is the fast one.) */
 int b200k_cache8_attention(void *out, const void *q, const int8_t *kc, const float *ks, const int8_t *vc,
                            const float *vs, const int32_t *tables, const int32_t *starts, const int32_t *lengths,
                            int32_t n, int32_t n_seqs, int32_t table_width, int32_t blocks, int32_t block, int32_t nh,

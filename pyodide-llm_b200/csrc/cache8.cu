@@ -35,7 +35,7 @@ __device__ __forceinline__ int over(int x, int by, uint32_t inverse) {
 // be updated in place, have to wait until every block has read them: the one cluster barrier.
 // Steps of more than ROWS_APART rows have them written by a second launch, on all SMs: 1000 requests of 64 tokens each take
 // 14 us so and 20 with the cluster writing them, 64 of 512 8 and 9, 64 of 64 (the bound's other side) 8 by one block.
-// Measured: 64 requests of a token each 6.4 us; 1000 that add 250 to 500 tokens each (358,000 rows) 16.5 us, of which the
+// Measured: 64 requests of a token each 5.8 us; 1000 that add 250 to 500 tokens each (358,000 rows) 15.8 us, of which the
 // sums over 1000 requests, by every block, are most. A launch by itself is 2 to 3 us.
 
 constexpr int TT = 512;  // threads, and the requests of one tile of the running sums
@@ -309,8 +309,9 @@ __global__ void __launch_bounds__(RT_THREADS) block_rows_kernel(TablesArgs a) {
 // where its run of tokens begins: no two teams touch one (block, head), and no atomics. A team is a thread block, or a
 // warp where the call has few tokens; it keeps the values that fit its registers between finding the largest and
 // rounding (the rest it reads again, from L1).
-// Measured with the load that follows, 8 heads of 128: 64 single tokens in float32 8.2 us (a thread block a token 9.5),
-// 4700 tokens of 64 prompts in float16 35 us, of which the load is 12 (a warp a run: 54 together). Bound by instructions
+// Measured with the load that follows, 8 heads of 128: 64 single tokens in float32 7.5 us (a thread block a token 9.5),
+// 4700 tokens of 64 prompts in float16 35 us where the rows are in L2, else 42, of which the load is 12 (a warp a run: 54
+// together). Bound by instructions
 // and their latency: a run's slots, scale and largest value come one after the other.
 
 constexpr int ST = 128;  // threads of a block

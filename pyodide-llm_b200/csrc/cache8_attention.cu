@@ -24,7 +24,7 @@
 // another. (Each lane copying what it will multiply itself, 64-byte runs of eight rows, read 4.5 TB/s, this 5.8.) The
 // pieces of a row are swapped about by its number, so that neither the keys' reads nor the values' collide in a bank.
 // Bound by reading the cache, and close behind by instructions. Measured, 32 query and 8 kv heads of 128: 64 requests of 512
-// to 8192 positions, float32, 104 us (0.55 GB at 5.3 TB/s, 0.81 of a copy's rate; the loads by themselves 99); one of 131071,
+// to 8192 positions, float32, 101 us (0.55 GB at 5.4 TB/s, 0.83 of a copy's rate; the loads by themselves 99); one of 131071,
 // float16, 58 us (4.6 TB/s: 0.27 GB are read in 41 us, and the first loads, the cut at the end and the joining are 17 more).
 #include <string>
 

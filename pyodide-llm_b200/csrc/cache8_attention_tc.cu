@@ -23,7 +23,7 @@
 // steps on average. Float32, heads of 64: 1550 a step of one tile (one warpgroup of softmax: 2060), of which the products
 // are about 900; each softmax step takes 2300 to 2600, twice its instructions' issue slots.
 // Measured: 8 requests that add 260 to 509 tokens to contexts of up to 4500, 32 query and 8 kv heads of 128, float16: 168 us
-// (0.66 PFLOP/s of what the masks leave); 4 whole prompts of 2048 tokens, 8 heads of 64, float32: 87 us.
+// (0.66 PFLOP/s of what the masks leave); 4 whole prompts of 2048 tokens, 8 heads of 64, float32: 90 us.
 // TMEM (512 columns), float16: tile t's two score buffers at 128 t + {0, 64}, its O at 256 + t * head size; float32: three
 // score buffers (heads of up to 64: four) at 64 u, two of O behind them.
 // Every wait is bounded: past it the kernel sets the scratch's error word (b200k_cache8_attention_check) and runs to its end.
