@@ -260,3 +260,11 @@ def test_attention_of_many_short_requests(requests):
     rng = np.random.default_rng(requests)
     c = Case([(int(rng.integers(1, 80)), int(rng.integers(0, 2))) for _ in range(requests)], 4, 2, 32, 16, False, seed=requests)
     check_exact(c)
+
+
+def test_attention_of_float16_gives_the_same_bits_again():
+    c = Case([(20000, 1), (900, 1), (130, 3), (700, 200)], 8, 2, 128, 32, True, seed=12)
+    first = c.run().copy()
+    for _ in range(5):
+        c.call()
+        assert np.array_equal(c.result(), first)
