@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, (Shape<HSEG, RT, HALF>::MINB)) cache8
               for (int e = 0; e < 4; e++) {
                 // q 2^29 = 2^24 d0 + 2^16 d1 + 2^8 d2 + d3, the digits from -128 to 127: with 128 added to the lower
                 // three, the bytes of the sum, less that
-                const uint32_t sum = (uint32_t)(__float2int_rn(z[e] * f[t] * 536870912.0f) + 0x808080) ^ 0x808080u;
+                const uint32_t sum = ((uint32_t)__float2int_rn(z[e] * f[t] * 536870912.0f) + 0x808080u) ^ 0x808080u;
 #pragma unroll
                 for (int k = 0; k < 4; k++) word[k][y] |= (sum >> (24 - 8 * k) & 255) << (8 * e);
               }
